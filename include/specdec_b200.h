@@ -266,6 +266,58 @@ int specdec_rmsnorm(const void* x, const void* residual, const void* weight, voi
 /* SiluAndMul (nanovllm/layers/activation.py:8-11): gate_up [T, 2 I] bf16 -> out [T, I] = silu(gate) * up. */
 int specdec_silu_mul(const void* gate_up, void* out, long long T, int intermediate, void* stream);
 
+/* ------------------------------------------------------------------------------------------ 8-bit K/V cache */
+/* store_kvcache (nanovllm/layers/attention.py:33-40) into an 8-bit paged cache: key / value [N][Hkv][128] bf16 (row
+ * strides in elements, multiples of 4) to slot_mapping [N] (any order; -1 skipped; a slot past the cache is skipped and
+ * sets *err = 3; a slot given twice holds its last token).  k_cache / v_cache [num_blocks][Hkv][block_size][128] e4m3,
+ * k_scale / v_scale [num_blocks][Hkv][block_size / scale_group] fp32, scale_group 16 or 32: an element stands for its
+ * code times its group's scale.  With a the largest finite magnitude that the call stores in a group and 2^e the
+ * smallest power of two >= 2^-100 with a <= 448 * 2^e: a call that writes the group's first slot sets the scale to 2^e;
+ * any other raises it to 2^e where that is larger, and requantises the group's other slots then.  Codes are rounded to
+ * nearest even, infinities saturate, NaN stays.  N <= 16384. */
+int specdec_store_kvcache_fp8(const void* key, long long key_row_stride, const void* value,
+                              long long value_row_stride, void* k_cache, void* v_cache, float* k_scale,
+                              float* v_scale, const int* slot_mapping, long long N, int num_kv_heads, int head_dim,
+                              long long num_blocks, int block_size, int scale_group, int* err, void* stream);
+
+/* specdec_paged_attention_ex over that cache (Attention.forward, nanovllm/layers/attention.py:59-77): the same row
+ * metadata, workspace (specdec_attention_workspace_bytes), flags and limits; q rows a multiple of 8 elements apart,
+ * caches and scales 16-byte aligned.  A query that sees no key gives zeros.  *err: 2 row metadata inconsistent with the
+ * block table width, 5 a block id outside the cache (read as block 0), 11 on a bounded wait gave up. */
+int specdec_paged_attention_fp8(const void* q, long long T, long long q_row_stride, int num_heads, int num_kv_heads,
+                                int head_dim, const void* k_cache, const void* v_cache, const float* k_scale,
+                                const float* v_scale, long long num_blocks, int block_size, int scale_group,
+                                const int* cu_seqlens_q, const int* cu_seqlens_k, const int* context_lens,
+                                int q_per_seq, int R, const int* block_tables, int W, int max_seqlen_q,
+                                float softmax_scale, int causal, void* out, long long out_row_stride, void* workspace,
+                                long long workspace_bytes, int* err, unsigned flags, void* stream);
+
+/* ------------------------------------------------------------------------------------------ round metadata */
+/* verify_varlen_metadata (nanovllm/engine/batch_metadata.py:121-181) on the GPU, the drafts placed among the input ids
+ * (nanovllm/engine/speculative.py:514-517) and the blocks that rows lack taken from a free stack
+ * (nanovllm/engine/scheduler.py:75-92).  lengths, last_tokens [R], drafts [R][k] (or null: ids 0), verified_lens [R] (or
+ * null: k + 1 each); block_tables [R][table_width] and num_blocks [R] in place: a row is extended to
+ * ceil((lengths - 1 + verified_lens) / block_size) blocks from the top of free_blocks[0 .. *free_count), rows in order,
+ * and *free_count lowered (both null: rows must hold what they need).  buf64 [2 num_tokens]: input ids, positions; buf32:
+ * slot_mapping [num_tokens], cu_seqlens_q, cu_seqlens_k [num_rows + 1], block_tables [num_rows][width], padding rows of
+ * at most k + 1 tokens on pad_block_id.  ticket: one zeroed word, left zero; calls sharing it must not overlap.  *err: 6
+ * the stack ran out, 7 a row argument out of range; such a call assigns nothing and leaves every row empty. */
+int specdec_verify_metadata(const long long* lengths, const long long* last_tokens, const long long* drafts,
+                            const long long* verified_lens, int R, int k, int* block_tables, int table_width,
+                            int* num_blocks, const int* free_blocks, int* free_count, int free_capacity,
+                            int block_size, int num_rows, int num_tokens, int pad_block_id, int width,
+                            long long* buf64, int* buf32, unsigned* ticket, int* err, void* stream);
+
+/* ------------------------------------------------------------------------------------------ log probabilities */
+/* What a server answers with beside the tokens (probs_from_logits, nanovllm/layers/spec_sampler.py:65-69, writes all
+ * T * V probabilities): for each row of logits [T][V] (dtype code, row stride in elements) divided by temperatures [T]
+ * (null: 1), logprobs[t] = log softmax at tokens[t], entropy[t] in nats, and the num_top (0 .. 32) largest logits' ids
+ * (ties to the lowest index, NaN above all) and log probabilities [T][num_top].  A negative token: the row is not read,
+ * 0, 0, ids -1, 0.  A token past V: NaN and *err = 8.  T <= 65535, V <= 2^24. */
+int specdec_token_logprobs(const void* logits, int dtype, long long T, long long V, long long row_stride,
+                           const long long* tokens, const float* temperatures, int num_top, float* logprobs,
+                           float* entropy, long long* top_ids, float* top_logprobs, int* err, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

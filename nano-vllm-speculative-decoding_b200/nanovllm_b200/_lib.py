@@ -81,6 +81,18 @@ SIGNATURES = {
                                           _c_void_p, _c_ll, _c_void_p, _c_ll, _c_void_p, _c_void_p, _c_void_p,
                                           _c_void_p, _c_ll, _c_ll, _c_float, _c_void_p, _c_ll, _c_void_p,
                                           _c_void_p]),
+    "specdec_store_kvcache_fp8": (_c_int, [_c_void_p, _c_ll, _c_void_p, _c_ll, _c_void_p, _c_void_p, _c_void_p,
+                                           _c_void_p, _c_void_p, _c_ll, _c_int, _c_int, _c_ll, _c_int, _c_int,
+                                           _c_void_p, _c_void_p]),
+    "specdec_paged_attention_fp8": (_c_int, [_c_void_p, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_void_p, _c_void_p,
+                                             _c_void_p, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p,
+                                             _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_float, _c_int,
+                                             _c_void_p, _c_ll, _c_void_p, _c_ll, _c_void_p, ctypes.c_uint, _c_void_p]),
+    "specdec_verify_metadata": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
+                                         _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                         _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "specdec_token_logprobs": (_c_int, [_c_void_p, _c_int, _c_ll, _c_ll, _c_ll, _c_void_p, _c_void_p, _c_int,
+                                        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lib = None

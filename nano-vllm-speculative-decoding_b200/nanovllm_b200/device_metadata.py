@@ -1,0 +1,85 @@
+"""A verification round's metadata built on the GPU from the requests' lengths.
+
+    verify_metadata(...)    batch_metadata.pack_verify_metadata and draft_placement (nanovllm/engine/batch_metadata.py:
+                            121-181, speculative.py:514-527) in one launch, the blocks that a row lacks taken from a free
+                            stack (scheduler.py:75-92)                                 -> specdec_verify_metadata
+
+The host form builds the arrays with numpy and copies them to the device three times a round; here the request state
+stays on the GPU (lengths, last tokens, drafts, block tables, the free blocks), so a round's metadata costs one launch and
+no host round trip.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import Workspace, check, ptr, require_cuda, stream_of
+from .batch_metadata import packed_sizes
+
+
+def _words(device: torch.device) -> torch.Tensor:
+    """[error word, ticket] of this device."""
+    return Workspace.get(device, 256, name="device_metadata")[:8].view(torch.int32)
+
+
+def device_error(device: torch.device) -> int:
+    """First error a verify_metadata call recorded on this device since the last reset (synchronises): 0 none, 6 the free
+    blocks ran out, 7 row arguments out of range (a verified length outside 1..k+1, a length below 1, a table too narrow
+    for the row, tokens that the padding rows cannot hold).  A call that records one assigns nothing and leaves every row
+    empty: cumulative lengths 0, slots -1."""
+    return int(_words(device)[0].item())
+
+
+def reset_device_error(device: torch.device) -> None:
+    _words(device)[0].zero_()
+
+
+def _of(name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor | None:
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {device} (got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device})")
+    return t
+
+
+def verify_metadata(lengths: torch.Tensor, last_tokens: torch.Tensor, drafts: torch.Tensor,
+                    verified_lens: torch.Tensor | None, block_tables: torch.Tensor, num_blocks: torch.Tensor,
+                    free_blocks: torch.Tensor | None, free_count: torch.Tensor | None, *, block_size: int, num_rows: int,
+                    num_tokens: int, pad_block_id: int, width: int, buf64: torch.Tensor, buf32: torch.Tensor) -> None:
+    """Writes the metadata of verifying R rows into the packed buffers buf64 / buf32 (batch_metadata.packed_views of
+    num_rows, num_tokens and width names their parts), the drafts placed among the input ids.
+
+    lengths, last_tokens [R] int64: a row's token count (its last token included, whose K/V are not stored yet) and that
+    token.  drafts [R, k] int64.  verified_lens [R] int64, 1..k+1 (None: k + 1 each); their sum and the tokens of the
+    padding rows (at most k + 1 each) make num_tokens.  block_tables [R, W'] int32 and num_blocks [R] int32: the blocks a
+    row holds, extended in place to what lengths - 1 + verified_lens tokens need with blocks from the top of the stack
+    free_blocks[:free_count] (int32, free_count [1] int32, lowered in place), rows in order.  Both None: the rows must
+    hold what they need.  The row arguments may be empty (R = 0): all padding.  Calls on one device share an error word and
+    a ticket: they must not overlap on the GPU."""
+    device = require_cuda(lengths, last_tokens, drafts, verified_lens, block_tables, num_blocks, free_blocks, free_count,
+                          buf64, buf32)
+    if drafts.dim() != 2 or block_tables.dim() != 2:
+        raise ValueError("drafts and block_tables must be 2-D")
+    R, k = drafts.shape
+    _of("lengths", lengths, torch.int64, (R,), device)
+    _of("last_tokens", last_tokens, torch.int64, (R,), device)
+    _of("drafts", drafts, torch.int64, (R, k), device)
+    _of("verified_lens", verified_lens, torch.int64, (R,), device)
+    _of("block_tables", block_tables, torch.int32, (R, block_tables.shape[1]), device)
+    _of("num_blocks", num_blocks, torch.int32, (R,), device)
+    if (free_blocks is None) != (free_count is None):
+        raise ValueError("give free_blocks and free_count together")
+    capacity = 0
+    if free_blocks is not None:
+        capacity = free_blocks.numel()
+        _of("free_blocks", free_blocks, torch.int32, (capacity,), device)
+        _of("free_count", free_count, torch.int32, (1,), device)
+    n64, n32 = packed_sizes(num_rows, num_tokens, width)
+    _of("buf64", buf64, torch.int64, (n64,), device)
+    _of("buf32", buf32, torch.int32, (n32,), device)
+    words = _words(device)
+    with torch.cuda.device(device):
+        check(_lib.lib().specdec_verify_metadata(
+            ptr(lengths), ptr(last_tokens), ptr(drafts), ptr(verified_lens), R, k, ptr(block_tables),
+            block_tables.shape[1], ptr(num_blocks), ptr(free_blocks), ptr(free_count), capacity, block_size, num_rows,
+            num_tokens, pad_block_id, width, ptr(buf64), ptr(buf32), words.data_ptr() + 4, words.data_ptr(),
+            stream_of(device)))

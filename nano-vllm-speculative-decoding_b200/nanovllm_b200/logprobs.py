@@ -1,0 +1,76 @@
+"""Log probabilities of given tokens, each position's entropy and its most likely tokens, in one pass over the logits.
+
+    token_logprobs(logits, tokens, num_top, temperatures)    -> specdec_token_logprobs
+
+Beside spec_sampler.probs_from_logits, which writes the whole [T, V] distribution: a server that answers with log
+probabilities wants a few numbers for each emitted token.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import DTYPE_CODES, Workspace, check, ptr, require_cuda, stream_of
+
+MAX_TOP = 32
+
+
+@dataclass
+class TokenLogprobs:
+    logprobs: torch.Tensor       # [T] fp32, log p of the given token
+    entropy: torch.Tensor        # [T] fp32, in nats
+    top_ids: torch.Tensor        # [T, num_top] int64, the most likely tokens, likeliest first
+    top_logprobs: torch.Tensor   # [T, num_top] fp32
+
+
+def _err_word(device: torch.device) -> torch.Tensor:
+    return Workspace.get(device, 256, name="logprobs")[:4].view(torch.int32)
+
+
+def device_error(device: torch.device) -> int:
+    """First error recorded on this device since the last reset (synchronises): 0 none, 8 a token id past the
+    vocabulary (its log probability is NaN)."""
+    return int(_err_word(device).item())
+
+
+def reset_device_error(device: torch.device) -> None:
+    _err_word(device).zero_()
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, num_top: int = 0,
+                   temperatures: torch.Tensor | None = None) -> TokenLogprobs:
+    """logits [T, V] (bf16, fp16 or fp32; rows may be strided), tokens [T] int64.  temperatures [T] fp32 > 0 (None: 1)
+    divide the logits first.  num_top (0 to 32, at most V) alternatives a row: the largest logits, ties to the lowest
+    index, NaN above every number.  Rows whose token is negative (padding) are not read: 0, 0, ids -1, 0.  A row with a
+    NaN or +inf, or nothing but -inf, has NaN for every log probability and the entropy; a single -inf is a token of
+    probability 0."""
+    device = require_cuda(logits, tokens, temperatures)
+    if logits.dim() != 2 or logits.dtype not in DTYPE_CODES:
+        raise ValueError(f"logits must be [T, V] bf16, fp16 or fp32 (got {logits.dtype} {tuple(logits.shape)})")
+    T, V = logits.shape
+    if tokens.shape != (T,):
+        raise ValueError(f"tokens {tuple(tokens.shape)} for {T} rows of logits")
+    if tokens.dtype.is_floating_point or tokens.dtype == torch.bool:
+        raise ValueError(f"tokens must be integers (got {tokens.dtype})")
+    if not 0 <= num_top <= min(MAX_TOP, V):
+        raise ValueError(f"num_top {num_top}: 0 to {MAX_TOP} and at most the vocabulary")
+    if temperatures is not None:
+        if temperatures.shape != (T,):
+            raise ValueError(f"temperatures {tuple(temperatures.shape)} for {T} rows of logits")
+        temperatures = temperatures.to(torch.float32).contiguous()
+    if T and (logits.stride(1) != 1 or (T > 1 and logits.stride(0) < V)):
+        logits = logits.contiguous()
+    stride = logits.stride(0) if T > 1 else V
+    tokens = tokens.to(torch.int64).contiguous()
+    out = TokenLogprobs(torch.empty(T, dtype=torch.float32, device=device),
+                        torch.empty(T, dtype=torch.float32, device=device),
+                        torch.empty(T, num_top, dtype=torch.int64, device=device),
+                        torch.empty(T, num_top, dtype=torch.float32, device=device))
+    with torch.cuda.device(device):
+        check(_lib.lib().specdec_token_logprobs(
+            ptr(logits), DTYPE_CODES[logits.dtype], T, V, stride, ptr(tokens), ptr(temperatures), num_top,
+            ptr(out.logprobs), ptr(out.entropy), ptr(out.top_ids), ptr(out.top_logprobs), ptr(_err_word(device)),
+            stream_of(device)))
+    return out

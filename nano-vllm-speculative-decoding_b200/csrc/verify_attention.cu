@@ -32,11 +32,9 @@
 // The softmax is online per query column with lazy rescaling (O is rescaled only when a column's running max
 // grows by more than 2^8), masked by key index (bottom-right causal or context length).  Keys past the row's
 // context in its last tile are never read as values: their P is 0 and their V rows are zeroed in shared memory.
-#include "common.cuh"
-#include "sm100.cuh"
+#include "paged_items.cuh"
 #include "specdec_b200.h"
 
-#include <cudaTypedefs.h>
 #include <math.h>
 #include <stddef.h>
 
@@ -45,10 +43,7 @@ namespace attention {
 
 using namespace sm100;
 
-constexpr int kHeadDim = 128;
-constexpr int kKeysPerTile = 128;
 constexpr int kSubKeys = 32;                              // an item's last tile loads in 32-key sub-boxes
-constexpr int kCols = 32;              // packed query columns (group x positions)
 constexpr int kStages = 3;             // K ring and V ring depth
 constexpr int kThreads = 384;            // warps 0-3: TMA (Q, K), MMA, prologue, TMA (V); 4-11: softmax
 constexpr int kHalfTileBytes = kKeysPerTile * 128;     // 64 dims x 128 keys bf16 = 16 KB
@@ -61,9 +56,6 @@ constexpr uint32_t kTmemCols = 128;                     // S0 | S1 | O0 | O1
 constexpr int kErrTimeoutQ = 11, kErrTimeoutK = 12, kErrTimeoutV = 13, kErrTimeoutS = 14, kErrTimeoutP = 15,
               kErrTimeoutO = 16, kErrTimeoutEmpty = 17;
 
-// One piece of a split item: O^T columns (unnormalised, relative to the piece's running maxima) then the maxima m
-// and the sums l of the 32 columns.
-constexpr int kPartialFloats = kCols * kHeadDim + 2 * kCols;
 constexpr int kMaxOuts = 8;            // output destinations of one launch (one per rank of an 8-GPU node)
 
 // Destinations beyond Args::out, written with the same offsets by the kPeers instantiation only (the peer-store
@@ -73,7 +65,6 @@ struct PeerOuts {
   __nv_bfloat16* out[kMaxOuts - 1];
   int n;                     // 0 .. kMaxOuts - 1
 };
-constexpr float kNegBig = -1.0e30f;    // start value of the running maxima (finite: no -inf arithmetic)
 
 struct Args {
   const int* cu_seqlens_q;   // [R + 1] or null (decode mode)
@@ -122,116 +113,6 @@ constexpr int kOffCtl = kOffP + 2 * kPBytes;
 constexpr int kSmemBytes = kOffCtl + (int)sizeof(Smem) + 1024;   // + alignment slack
 static_assert(kSmemBytes <= 232448, "shared memory above the sm_100 per-CTA limit");
 
-// Max over the warp's 32 lanes in one instruction (sm_100a redux.sync on f32).
-__device__ __forceinline__ float warp_max_redux(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-// Sum over the 32 lanes of 16 columns held by every lane; lane j ends with column (j & 15)'s sum; v is consumed.
-__device__ __forceinline__ float column_reduce16(float (&v)[16], int lane) {
-#pragma unroll
-  for (int c = 0; c < 16; ++c) v[c] += __shfl_xor_sync(0xffffffffu, v[c], 16);
-#pragma unroll
-  for (int w = 8; w >= 1; w >>= 1) {
-    const bool upper = (lane & w) != 0;
-#pragma unroll
-    for (int c = 0; c < w; ++c) {
-      const float send = upper ? v[c] : v[c + w];
-      const float keep = upper ? v[c + w] : v[c];
-      v[c] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-    }
-  }
-  return v[0];
-}
-
-// A row's queries and keys; nt = 0 when the row has no work (no queries, or metadata that the kernel rejects).
-struct RowInfo {
-  int q_start, ql, L, nt;
-};
-
-template <int QMAX>
-__device__ __forceinline__ RowInfo row_info(const Args& a, int b, bool report) {
-  RowInfo r;
-  if (a.cu_seqlens_q) {
-    r.q_start = a.cu_seqlens_q[b];
-    r.ql = a.cu_seqlens_q[b + 1] - r.q_start;
-    r.L = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b];
-  } else {
-    r.q_start = b * a.q_per_seq;
-    r.ql = a.q_per_seq;
-    r.L = a.context_lens[b];
-  }
-  r.nt = 0;
-  if (r.ql > 0) {
-    if (r.ql > QMAX || r.L <= 0 || r.L > a.W * a.block_size) {   // inconsistent metadata: report, never read
-      if (report) atomicCAS(a.err, 0, 2);
-    } else {
-      r.nt = (r.L + kKeysPerTile - 1) / kKeysPerTile;
-    }
-  }
-  return r;
-}
-
-// The item sequence: items (row b, KV head h) in row-major order, item (b, h) holding the sequence's tiles
-// [A, A + r.nt).  Each role of a CTA walks it from the item holding x_begin to the one holding x_end - 1.
-template <int QMAX>
-struct Walk {
-  int b, h;
-  long long A;
-  RowInfo r;
-  __device__ __forceinline__ void start(const Args& a, const Smem& S) {
-    b = S.b_start;
-    r = RowInfo{S.r0[0], S.r0[1], S.r0[2], S.r0[3]};   // found by the prologue
-    h = (int)((S.x_begin - S.row_tile0) / r.nt);
-    A = S.row_tile0 + (long long)h * r.nt;
-  }
-  __device__ __forceinline__ void next(const Args& a) {
-    A += r.nt;
-    if (++h == a.Hkv) {
-      h = 0;
-      do {
-        ++b;
-        r = b < a.R ? row_info<QMAX>(a, b, false) : RowInfo{0, 0, 0, 1};
-      } while (r.nt == 0);
-    }
-  }
-  // this CTA's tiles of the item: item-local [t0, t1)
-  __device__ __forceinline__ int t0(long long x_begin) const { return (int)(x_begin > A ? x_begin - A : 0); }
-  __device__ __forceinline__ int t1(long long x_end) const {
-    return (int)(x_end < A + r.nt ? x_end - A : (long long)r.nt);
-  }
-};
-
-// Tile-by-tile cursor over the CTA's share: the segment (item piece) index n of the current tile and whether the
-// tile is the segment's first / last.
-template <int QMAX>
-struct Cursor {
-  Walk<QMAX> w;
-  int n, left;
-  bool first;
-  __device__ __forceinline__ void start(const Args& a, const Smem& S) {
-    w.start(a, S);
-    n = 0;
-    left = w.t1(S.x_end) - w.t0(S.x_begin);
-    first = true;
-  }
-  __device__ __forceinline__ bool last() const { return left == 1; }
-  __device__ __forceinline__ void advance(const Args& a, long long x_begin, long long x_end) {
-    if (--left == 0) {
-      w.next(a);
-      ++n;
-      left = w.t1(x_end) - w.t0(x_begin);
-      first = true;
-    } else {
-      first = false;
-    }
-  }
-};
-
-__device__ __forceinline__ long long ceil_div(long long x, long long y) { return (x + y - 1) / y; }
-
 template <int G, bool kPeers>
 __global__ void __launch_bounds__(kThreads, 1)
     verify_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -279,49 +160,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&vmap32);
   }
   if (warp == 2) {
-    // ---- this CTA's share: the tile sequence split evenly over min(grid, tiles) CTAs, then the row holding
-    // its first tile (two passes of 32 rows at a time over the row metadata)
-    long long row_tiles = 0;
-    for (int b0 = 0; b0 < a.R; b0 += 32) {
-      const int b = b0 + lane;
-      const int nt = b < a.R ? row_info<QMAX>(a, b, true).nt : 0;
-      row_tiles += __reduce_add_sync(0xffffffffu, (unsigned)nt);
-    }
-    const long long T = row_tiles * a.Hkv;
-    const long long Ge = T < (long long)gridDim.x ? T : (long long)gridDim.x;
-    const long long c = blockIdx.x;
-    long long xb = 0, xe = 0, row0 = 0;
-    int bstart = 0, slot0 = 0;
-    RowInfo r0{0, 0, 0, 1};
-    if (c < Ge) {
-      xb = T * c / Ge;
-      xe = T * (c + 1) / Ge;
-      long long pre = 0;
-      for (int b0 = 0; b0 < a.R; b0 += 32) {
-        const int b = b0 + lane;
-        const RowInfo ri = b < a.R ? row_info<QMAX>(a, b, false) : RowInfo{0, 0, 0, 0};
-        const long long v = (long long)ri.nt * a.Hkv;
-        long long inc = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += y;
-        }
-        const long long first = pre + inc - v;
-        const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && xb >= first && xb < first + v);
-        if (hit) {
-          const int src = __ffs(hit) - 1;
-          bstart = b0 + src;
-          row0 = __shfl_sync(0xffffffffu, first, src);
-          r0.q_start = __shfl_sync(0xffffffffu, ri.q_start, src);
-          r0.ql = __shfl_sync(0xffffffffu, ri.ql, src);
-          r0.L = __shfl_sync(0xffffffffu, ri.L, src);
-          r0.nt = __shfl_sync(0xffffffffu, ri.nt, src);
-          break;
-        }
-        pre += __shfl_sync(0xffffffffu, inc, 31);
-      }
-    }
+    // ---- this CTA's share of the tile sequence and the row holding its first tile
+    const Share share = find_share<QMAX>(a, lane);
+    const long long T = share.T, Ge = share.Ge, c = blockIdx.x, xb = share.xb, xe = share.xe, row0 = share.row0;
+    const int bstart = share.bstart;
+    const RowInfo r0 = share.r0;
+    int slot0 = 0;
     if (c < Ge && lane == 0) {       // the share's first tile: its key in the row and its cache slot
       const long long h = (xb - row0) / r0.nt;
       const int key0 = (int)(xb - row0 - h * r0.nt) * kKeysPerTile;
@@ -746,20 +590,6 @@ __global__ void __launch_bounds__(256) store_kv_kernel(const __nv_bfloat16* key,
 }
 
 // ---------------------------------------------------------------------------------------- host side
-// The driver's tensor-map encoder (one entry point for every device), looked up on first use; the initialisation
-// of a function-local static is thread-safe.
-static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    return nullptr;
-  }();
-  return fn;
-}
-
 // 3-D bf16 tensor map (dim0 contiguous), 128-byte swizzle, box {64, box1, box2}.
 static int make_map(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
                     uint64_t stride2_bytes, uint32_t box1, uint32_t box2) {
@@ -798,16 +628,6 @@ static int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
   SPECDEC_LAUNCH_CHECK();
   return kOk;
 }
-
-// Workspace: two piece slots per SM (a size fixed per device), then R * Hkv arrival counters (256-byte padded).
-// The counters sit at the same offset for calls of every shape, so a workspace zeroed once stays valid: every
-// call leaves the counters it used at zero, and no call's pieces overlap another call's counters.
-static long long partial_bytes(int sm_count) { return 2LL * sm_count * kPartialFloats * 4; }
-static long long counters_bytes(long long R, int Hkv) { return (R * Hkv * 4 + 255) / 256 * 256; }
-static long long workspace_bytes(long long R, int Hkv, int sm_count) {
-  return partial_bytes(sm_count) + counters_bytes(R, Hkv);
-}
-static_assert((kPartialFloats * 4 * 2) % 256 == 0, "counters stay 256-byte aligned");
 
 }  // namespace attention
 }  // namespace specdec

@@ -1,11 +1,36 @@
-// Verify / decode attention over the 8-bit paged cache (e4m3 codes, a scale per group of slots and KV head).
+// Verify / decode attention over the 8-bit paged cache (e4m3 codes, a scale per group of slots and KV head) for sm_100a.
 //
-// Reference behaviour: Attention.forward, verify and decode branches (nanovllm/layers/attention.py:59-77), over a
-// cache whose keys and values are code * scale:
-//   o = sum_j softmax_j(softmax_scale * ks_j * (q . k_j)) * vs_j * v_j.
+// Reference behaviour: Attention.forward, verify and decode branches (nanovllm/layers/attention.py:59-77), over keys and
+// values that are code * scale:
+//   o = sum_j p_j vs_j v_j,  p = softmax_j(softmax_scale * ks_j * (q . k_j)),
+// causal (bottom-right aligned) or over the whole context; a query that sees no key gives zeros.
 //
-// First form: a warp per (token, query head) walks the row's keys with a running maximum and sum, 4 dims a lane.
-#include "common.cuh"
+// What bounds it: HBM.  A 128-key tile of one head is 2 * 16 KB of codes (half the bf16 cache's) and 64 B of scales for
+// 4 * 128 * 128 * 32 FLOP, 128 FLOP a byte.  The cache's layout keeps a head's rows of a block together, so a tile is one
+// contiguous 16 KB.
+//
+// Design.  The item sequence, its split over a persistent grid and the merge of split items are the bf16 kernel's
+// (paged_items.cuh, verify_attention.cu).  What differs is how 8-bit codes meet the tensor core without being widened in
+// shared memory (widening a tile would cost a read of 32 KB and a write of 64 KB of shared memory a tile, more than the
+// 748 ns that HBM leaves it):  the MMAs are kind::f8f6f4 with the cache's codes as the A operand straight from the TMA's
+// tile, and the other operand, which is 16-bit by nature, goes in as a sum of 8-bit parts side by side in N:
+//   S^T[128 keys x 2*32] = K . [q1 | q2]^T   q = 2^e (q1 + q2 / 16), both e4m3: bf16's 8 bits are 4 + 4, so the split is
+//                                            exact down to 2^-14 of the item's largest query element (beyond: an absolute
+//                                            2^-22 of it), e from that element
+//   O^T[128 dims x 3*32] += V^T . [p1 | p2 | p3]^T   p = p1 + p2 + p3, all e5m2: 3 bits each, p to 2^-9 of itself (what
+//                                            bf16 gives) down to 2^-24 of the column's running maximum (e5m2's range)
+// N-wise parts read A once; stacked along K they would read it 2 and 3 times, and A's reads of shared memory are what an
+// MMA with so few columns costs.  The parts' sums are taken in fp32 after TMEM.
+// The scales never touch the codes: ks_j multiplies the score, and vs_j goes into the exponent: with t_j = s_j + log2 vs_j
+// the running maximum is over t, the tensor core gets p'_j = 2^(t_j - m) (so the largest contribution keeps every bit
+// whatever the scales' spread), and the denominator sums p'_j / vs_j.
+//   warp 0       TMA producer: the K tiles             warps 4-11   softmax over keys (a TMEM lane is a key; two groups of
+//   warp 1       TMEM allocator, MMA issuer                          16 columns each), P parts, O rescale, epilogue
+//   warp 2       prologue; producer of the scales      warps 12-15  query parts of the next items; rows without keys
+//   warp 3       TMA producer: the V tiles
+// Softmax: online per column with lazy rescaling (O is rescaled when a column's maximum grows by more than 2^8; p' reaches
+// 2^15 then, in e5m2's range), masked by key index.  V rows past the context are zeroed in shared memory.
+#include "paged_items.cuh"
 #include "specdec_b200.h"
 
 #include <cuda_fp8.h>
@@ -14,85 +39,647 @@
 namespace specdec {
 namespace attention_fp8 {
 
-constexpr int kHeadDim = 128;
-constexpr int kCols = 32;
-constexpr int kKeysPerTile = 128;
+using namespace attention;
+
+constexpr int kSubKeys = 32;                          // an item's last tile loads in 32-key sub-boxes
+constexpr int kStages = 5;                            // K ring and V ring depth: 160 KB in flight
+constexpr int kScaleStages = 8;                       // scale ring depth
+constexpr int kThreads = 512;
+constexpr int kTileBytes = kKeysPerTile * kHeadDim;   // 16 KB of codes
+constexpr int kQParts = 2, kPParts = 3;
+constexpr int kQBytes = kQParts * kCols * kHeadDim;   // 8 KB, double-buffered by item
+constexpr int kPPartBytes = kKeysPerTile * kCols;     // 4 KB
+constexpr int kPBytes = kPParts * kPPartBytes;        // 12 KB, double-buffered by tile
+constexpr uint32_t kTmemCols = 512;                   // S0 at 0, S1 at 64; O0 at 128, O1 at 256 (96 columns each)
+constexpr uint32_t kTmemO = 128, kTmemOStride = 128;
+constexpr float kPBias = 7.0f;                        // p' is kept 2^7 up: its range is [2^-24, 2^8] of the maximum
+constexpr float kMinScale = 7.888609052210118e-31f;   // 2^-100, the store's smallest scale
+
+constexpr int kErrTimeoutQ = 11, kErrTimeoutK = 12, kErrTimeoutV = 13, kErrTimeoutS = 14, kErrTimeoutP = 15,
+              kErrTimeoutO = 16, kErrTimeoutEmpty = 17, kErrTimeoutScale = 18, kErrPage = 5;
 
 struct Args {
-  const __nv_bfloat16* q;
+  const __nv_bfloat16* q;    // [T, H, D]
   long long q_row_stride;
-  const unsigned char *k_cache, *v_cache;
   const float *k_scale, *v_scale;
-  const int *cu_seqlens_q, *cu_seqlens_k, *context_lens;
-  int q_per_seq, R, max_q;
-  const int* block_tables;
+  const int* cu_seqlens_q;   // [R + 1] or null (decode mode)
+  const int* cu_seqlens_k;
+  const int* context_lens;   // [R] (decode mode)
+  int q_per_seq, R, T;
+  const int* block_tables;   // [R, W]
   int W, block_size, group;
-  long long num_blocks;
+  int num_blocks;
   int H, Hkv;
-  float scale;
+  float scale_log2;          // softmax_scale * log2(e)
   int causal;
   __nv_bfloat16* out;
   long long out_row_stride;
+  int* counters;
+  float* partial;
   int* err;
 };
 
-__device__ __forceinline__ float4 decode4(unsigned c) {
-  const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xffffu), __NV_E4M3)));
-  const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16), __NV_E4M3)));
-  return make_float4(lo.x, lo.y, hi.x, hi.y);
+struct Smem {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t sc_full[kScaleStages], sc_empty[kScaleStages];
+  uint64_t s_full[2], s_free[2], p_full[2], o_done[2], o_free[2];
+  alignas(16) float scales[kScaleStages][2][kKeysPerTile / 16];   // [ring][K, V][group of the tile]
+  alignas(16) float red_max[2][32][4];   // [tile parity][column][warp] maxima
+  alignas(16) float red_sum[32][4];
+  unsigned red_q[4];
+  float q_scale[4];          // by item & 3: the item's 2^e
+  uint32_t tmem_base;
+  int abort;
+  long long total_tiles, x_begin, x_end, row_tile0;
+  int b_start, active;
+  int r0[4];
+  int page0;                 // page of the share's first tile
+  int last_piece;
+};
+
+constexpr int kOffQ = 0;
+constexpr int kOffK = kOffQ + 2 * kQBytes;
+constexpr int kOffV = kOffK + kStages * kTileBytes;
+constexpr int kOffP = kOffV + kStages * kTileBytes;
+constexpr int kOffCtl = kOffP + 2 * kPBytes;
+constexpr int kSmemBytes = kOffCtl + (int)sizeof(Smem) + 1024;   // + alignment slack
+static_assert(kSmemBytes <= 232448, "shared memory above the sm_100 per-CTA limit");
+
+__device__ __forceinline__ float2 decode_e4m3x2(unsigned pair) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3)));
+}
+__device__ __forceinline__ unsigned encode_e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ unsigned encode_e5m2x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E5M2);
+}
+// The value with its mantissa cut to e5m2's two bits (towards zero).
+__device__ __forceinline__ float cut3(float x) { return __uint_as_float(__float_as_uint(x) & 0xffe00000u); }
+
+// The page of a row's key, block 0 in place of an id outside the cache.
+__device__ __forceinline__ int page_of(const Args& a, const int* table, int key0) {
+  int page = table[key0 / a.block_size];
+  if (page < 0 || page >= a.num_blocks) {
+    atomicCAS(a.err, 0, kErrPage);
+    page = 0;
+  }
+  return page;
 }
 
-__global__ void __launch_bounds__(256) simple_kernel(const Args a) {
-  const int b = blockIdx.x, lane = threadIdx.x & 31;
-  int q0, ql, L;
-  if (a.cu_seqlens_q) {
-    q0 = a.cu_seqlens_q[b];
-    ql = a.cu_seqlens_q[b + 1] - q0;
-    L = a.cu_seqlens_k[b + 1] - a.cu_seqlens_k[b];
-  } else {
-    q0 = b * a.q_per_seq;
-    ql = a.q_per_seq;
-    L = a.context_lens[b];
-  }
-  if (ql <= 0) return;
-  if (ql > a.max_q || L < 0 || L > a.W * a.block_size) {
-    if (threadIdx.x == 0) atomicCAS(a.err, 0, 2);
-    return;
-  }
-  for (int u = blockIdx.y * 8 + (threadIdx.x >> 5); u < ql * a.H; u += gridDim.y * 8) {
-    const int p = u / a.H, head = u % a.H, h = head / (a.H / a.Hkv);
-    const uint2 qq = *reinterpret_cast<const uint2*>(a.q + (long long)(q0 + p) * a.q_row_stride + head * kHeadDim + lane * 4);
-    const float qf[4] = {__uint_as_float(qq.x << 16), __uint_as_float(qq.x & 0xffff0000u), __uint_as_float(qq.y << 16),
-                         __uint_as_float(qq.y & 0xffff0000u)};
-    const int limit = a.causal ? min(L, L - ql + p + 1) : L;
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int key = 0; key < limit; ++key) {
-      const long long block = a.block_tables[(long long)b * a.W + key / a.block_size];
-      if (block < 0 || block >= a.num_blocks) {
-        if (lane == 0) atomicCAS(a.err, 0, 5);
-        continue;
-      }
-      const long long bh = block * a.Hkv + h;
-      const int j = key % a.block_size;
-      const long long at = (bh * a.block_size + j) * kHeadDim + lane * 4;
-      const long long sat = bh * (a.block_size / a.group) + j / a.group;
-      const float4 k = decode4(*reinterpret_cast<const unsigned*>(a.k_cache + at));
-      const float4 v = decode4(*reinterpret_cast<const unsigned*>(a.v_cache + at));
-      const float s = warp_sum_f32(qf[0] * k.x + qf[1] * k.y + qf[2] * k.z + qf[3] * k.w) * a.k_scale[sat] * a.scale;
-      const float vs = a.v_scale[sat], mn = fmaxf(m, s), c = expf(m - mn), pr = expf(s - mn);
-      m = mn;
-      l = l * c + pr;
-      o[0] = o[0] * c + pr * vs * v.x;
-      o[1] = o[1] * c + pr * vs * v.y;
-      o[2] = o[2] * c + pr * vs * v.z;
-      o[3] = o[3] * c + pr * vs * v.w;
+template <int G>
+__global__ void __launch_bounds__(kThreads, 1)
+    verify_attention_fp8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                const __grid_constant__ CUtensorMap kmap32, const __grid_constant__ CUtensorMap vmap32,
+                                const Args a) {
+  constexpr int QMAX = kCols / G;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* sQ = base + kOffQ;
+  unsigned char* sK = base + kOffK;
+  unsigned char* sV = base + kOffV;
+  unsigned char* sP = base + kOffP;
+  Smem& S = *reinterpret_cast<Smem*>(base + kOffCtl);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S.q_full[i], 4);     // one elected arrival per query warp
+      mbar_init(&S.q_empty[i], 1);
+      mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.s_free[i], 8);     // one per softmax warp
+      mbar_init(&S.p_full[i], 8);
+      mbar_init(&S.o_done[i], 1);
+      mbar_init(&S.o_free[i], 8);
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    __nv_bfloat162* dst =
-        reinterpret_cast<__nv_bfloat162*>(a.out + (long long)(q0 + p) * a.out_row_stride + head * kHeadDim + lane * 4);
-    dst[0] = __floats2bfloat162_rn(o[0] * inv, o[1] * inv);
-    dst[1] = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&S.k_full[s], 1);
+      mbar_init(&S.k_empty[s], 1);
+      mbar_init(&S.v_full[s], 1);
+      mbar_init(&S.v_empty[s], 1);
+    }
+    for (int s = 0; s < kScaleStages; ++s) {
+      mbar_init(&S.sc_full[s], 1);
+      mbar_init(&S.sc_empty[s], 8);
+    }
+    S.abort = 0;
+    fence_barrier_init();
   }
+  if (warp == 1) {
+    tmem_alloc(&S.tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+    prefetch_tensormap(&kmap32);
+    prefetch_tensormap(&vmap32);
+  }
+  if (warp == 2) {
+    const Share share = find_share<QMAX, true>(a, lane);
+    if (lane == 0) {
+      int page0 = 0;
+      if (share.xe > share.xb) {       // the share's first tile: its page, and its codes into L2 ahead of the loads
+        const int h = (int)((share.xb - share.row0) / share.r0.nt);
+        const int key0 = (int)(share.xb - share.row0 - (long long)h * share.r0.nt) * kKeysPerTile;
+        page0 = page_of(a, a.block_tables + (long long)share.bstart * a.W, key0);
+        tma_prefetch_3d(&kmap, 0, key0 % a.block_size, page0 * a.Hkv + h);
+        tma_prefetch_3d(&vmap, 0, key0 % a.block_size, page0 * a.Hkv + h);
+      }
+      S.total_tiles = share.T;
+      S.active = (int)share.Ge;
+      S.x_begin = share.xb;
+      S.x_end = share.xe;
+      S.row_tile0 = share.row0;
+      S.b_start = share.bstart;
+      S.r0[0] = share.r0.q_start;
+      S.r0[1] = share.r0.ql;
+      S.r0[2] = share.r0.L;
+      S.r0[3] = share.r0.nt;
+      S.page0 = page0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // an early (programmatic dependent) launch ran the prologue while the preceding kernel finished
+  griddep_wait();
+  const uint32_t tmem = S.tmem_base;
+  volatile int* abort = &S.abort;
+  const long long x_begin = S.x_begin, x_end = S.x_end;
+  const int ntiles = (int)(x_end - x_begin);
+
+  if (warp == 0 || warp == 3) {
+    // ------------------------------------------------------------------ TMA producers of the codes
+    const bool is_k = warp == 0;
+    if (lane == 0 && ntiles > 0) {
+      uint64_t* full = is_k ? S.k_full : S.v_full;
+      uint64_t* empty = is_k ? S.k_empty : S.v_empty;
+      unsigned char* ring = is_k ? sK : sV;
+      const CUtensorMap* map = is_k ? &kmap : &vmap;
+      const CUtensorMap* map32 = is_k ? &kmap32 : &vmap32;
+      Walk<QMAX, true> wk;
+      wk.start(a, S);
+      bool ok = true;
+      int g = 0;
+      for (; ok && wk.A < x_end; wk.next(a)) {
+        const int* table = a.block_tables + (long long)wk.b * a.W;
+        const int t1 = wk.t1(x_end);
+        for (int t = wk.t0(x_begin); t < t1; ++t, ++g) {
+          const int stage = g % kStages;
+          const uint32_t use = g / kStages;
+          const int key0 = t * kKeysPerTile;
+          const int page = g == 0 ? S.page0 : page_of(a, table, key0);
+          const int j0 = key0 % a.block_size, ph = page * a.Hkv + wk.h;
+          if (g >= kStages && !mbar_wait(&empty[stage], (use - 1) & 1, abort, a.err, kErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          const int subs = t == wk.r.nt - 1 ? (wk.r.L - key0 + kSubKeys - 1) / kSubKeys : kKeysPerTile / kSubKeys;
+          unsigned char* dst = ring + stage * kTileBytes;
+          mbar_arrive_expect_tx(&full[stage], subs * kSubKeys * kHeadDim);
+          if (subs == kKeysPerTile / kSubKeys) {
+            tma_load_3d(dst, map, 0, j0, ph, &full[stage]);
+          } else {
+            for (int j = 0; j < subs; ++j)
+              tma_load_3d(dst + j * kSubKeys * kHeadDim, map32, 0, j0 + j * kSubKeys, ph, &full[stage]);
+          }
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ producer of the scales
+    if (lane == 0 && ntiles > 0) {
+      const int per_tile = kKeysPerTile / a.group, per_block = a.block_size / a.group;
+      const uint32_t bytes = per_tile * 4;
+      Walk<QMAX, true> wk;
+      wk.start(a, S);
+      bool ok = true;
+      int g = 0;
+      for (; ok && wk.A < x_end; wk.next(a)) {
+        const int* table = a.block_tables + (long long)wk.b * a.W;
+        const int t1 = wk.t1(x_end);
+        for (int t = wk.t0(x_begin); t < t1; ++t, ++g) {
+          const int e = g % kScaleStages;
+          const int key0 = t * kKeysPerTile;
+          const int page = g == 0 ? S.page0 : page_of(a, table, key0);
+          const long long at =
+              ((long long)page * a.Hkv + wk.h) * per_block + key0 % a.block_size / kKeysPerTile * per_tile;
+          if (g >= kScaleStages &&
+              !mbar_wait(&S.sc_empty[e], (g / kScaleStages - 1) & 1, abort, a.err, kErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&S.sc_full[e], 2 * bytes);
+          bulk_load(S.scales[e][0], a.k_scale + at, bytes, &S.sc_full[e]);
+          bulk_load(S.scales[e][1], a.v_scale + at, bytes, &S.sc_full[e]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && ntiles > 0) {
+      const uint32_t idesc_s = idesc_f8_f32(128, kQParts * kCols, 0, 0, 0, 0);    // e4m3 . e4m3
+      const uint32_t idesc_o = idesc_f8_f32(128, kPParts * kCols, 0, 1, 1, 1);    // e4m3 . e5m2
+      Cursor<QMAX, true> cs, cp;     // the score MMAs run two tiles ahead of the PV MMAs
+      cs.start(a, S);
+      cp.start(a, S);
+      auto issue_s = [&](int g) -> bool {
+        const int stage = g % kStages;
+        const int qb = cs.n & 1;
+        if (cs.first && !mbar_wait(&S.q_full[qb], (cs.n >> 1) & 1, abort, a.err, kErrTimeoutQ)) return false;
+        if (!mbar_wait(&S.k_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutK)) return false;
+        if (g >= 2 && !mbar_wait(&S.s_free[g & 1], ((g - 2) >> 1) & 1, abort, a.err, kErrTimeoutS)) return false;
+        tc_fence_after();
+        const unsigned char* kt = sK + stage * kTileBytes;
+        const unsigned char* qt = sQ + qb * kQBytes;
+        const uint32_t tmem_s = tmem + (g & 1) * 64;
+#pragma unroll
+        for (int kk = 0; kk < kHeadDim / 32; ++kk) {
+          const uint64_t adesc = smem_desc(kt + kk * 32, 16, 1024, kSwizzle128B);
+          const uint64_t bdesc = smem_desc(qt + kk * 32, 16, 1024, kSwizzle128B);
+          mma_f8_ss(tmem_s, adesc, bdesc, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(&S.s_full[g & 1]);
+        mma_commit(&S.k_empty[stage]);
+        if (cs.last()) mma_commit(&S.q_empty[qb]);
+        cs.advance(a, x_begin, x_end);
+        return true;
+      };
+      auto issue_pv = [&](int g) -> bool {
+        const int stage = g % kStages;
+        const int ob = cp.n & 1;
+        if (cp.first && cp.n >= 2 && !mbar_wait(&S.o_free[ob], ((cp.n - 2) >> 1) & 1, abort, a.err, kErrTimeoutO))
+          return false;
+        if (!mbar_wait(&S.p_full[g & 1], (g >> 1) & 1, abort, a.err, kErrTimeoutP)) return false;
+        if (!mbar_wait(&S.v_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutV)) return false;
+        tc_fence_after();
+        const unsigned char* vt = sV + stage * kTileBytes;
+        const unsigned char* pt = sP + (g & 1) * kPBytes;
+        const uint32_t tmem_o = tmem + kTmemO + ob * kTmemOStride;
+        const bool fresh = cp.first;
+#pragma unroll
+        for (int kk = 0; kk < kKeysPerTile / 32; ++kk) {
+          const uint64_t adesc = smem_desc(vt + kk * 32 * kHeadDim, kTileBytes, 1024, kSwizzle128B);
+          const uint64_t bdesc = smem_desc(pt + kk * 32 * kCols, kPPartBytes, 256, kSwizzle32B);
+          mma_f8_ss(tmem_o, adesc, bdesc, idesc_o, (!fresh || kk > 0) ? 1u : 0u);
+        }
+        mma_commit(&S.o_done[g & 1]);
+        mma_commit(&S.v_empty[stage]);
+        cp.advance(a, x_begin, x_end);
+        return true;
+      };
+      bool ok = issue_s(0);
+      if (ok && ntiles > 1) ok = issue_s(1);
+      for (int g = 0; g < ntiles && ok; ++g) {
+        if (g + 2 < ntiles) ok = issue_s(g + 2);
+        if (ok) ok = issue_pv(g);
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------ query parts: 32 columns x 128 dims an item
+    // a column's 128 dims belong to four threads, 32 each
+    const int tid = threadIdx.x - 384, col = tid >> 2, quarter = tid & 3;
+    const int p = col / G, gq = col % G;
+    if (ntiles > 0) {
+      Walk<QMAX, true> wk;
+      wk.start(a, S);
+      for (int n = 0; wk.A < x_end; wk.next(a), ++n) {
+        uint4 raw[4];
+        unsigned most = 0;
+        const uint4* src = reinterpret_cast<const uint4*>(
+            a.q + (long long)(wk.r.q_start + p) * a.q_row_stride + (wk.h * G + gq) * kHeadDim + quarter * 32);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = p < wk.r.ql ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+          }
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        named_barrier(4, 128);                 // the last item's maxima have been read
+        if (lane == 0) S.red_q[warp - 12] = most;
+        named_barrier(4, 128);
+        most = max(max(S.red_q[0], S.red_q[1]), max(S.red_q[2], S.red_q[3]));
+        // 2^e with every |q| <= 448 * 2^e = 1.75 * 2^(e + 8)
+        int e = (int)(most >> 7) - 135 + ((most & 0x7fu) > 0x60u ? 1 : 0);
+        e = max(e, -100);
+        const float inv = __uint_as_float((unsigned)(127 - e) << 23);
+        if (n >= 2 && !mbar_wait(&S.q_empty[n & 1], ((n - 2) >> 1) & 1, abort, a.err, kErrTimeoutEmpty)) break;
+        unsigned char* q1 = sQ + (n & 1) * kQBytes + col * 128;
+        unsigned char* q2 = q1 + kCols * 128;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {       // 16 dims: one 16-byte chunk of each part
+          unsigned b1[8], b2[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint4& r4 = raw[i + k / 4];
+            const unsigned w = k % 4 == 0 ? r4.x : k % 4 == 1 ? r4.y : k % 4 == 2 ? r4.z : r4.w;
+            float x = __uint_as_float(w << 16) * inv, y = __uint_as_float(w & 0xffff0000u) * inv;
+            x += x - x;                        // infinities become NaN (a saturating conversion would hide them)
+            y += y - y;
+            b1[k] = encode_e4m3x2(x, y);
+            const float2 d = decode_e4m3x2(b1[k]);
+            b2[k] = encode_e4m3x2((x - d.x) * 16.0f, (y - d.y) * 16.0f);
+          }
+          const int phys = ((quarter * 2 + i / 2) ^ (col & 7)) * 16;
+          *reinterpret_cast<uint4*>(q1 + phys) = make_uint4(b1[0] | b1[1] << 16, b1[2] | b1[3] << 16,
+                                                            b1[4] | b1[5] << 16, b1[6] | b1[7] << 16);
+          *reinterpret_cast<uint4*>(q2 + phys) = make_uint4(b2[0] | b2[1] << 16, b2[2] | b2[3] << 16,
+                                                            b2[4] | b2[5] << 16, b2[6] | b2[7] << 16);
+        }
+        // read by the softmax before it frees the item's first score tile; written again four items on, after that
+        if (tid == 0) S.q_scale[n & 3] = __uint_as_float((unsigned)(e + 127) << 23);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.q_full[n & 1]);
+      }
+    }
+    // rows of queries without a key: zeros
+    for (int b = blockIdx.x; b < a.R; b += gridDim.x) {
+      const RowInfo r = row_info<QMAX, true>(a, b, false);
+      if (r.ql <= 0 || r.ql > QMAX || r.L != 0) continue;
+      const int chunks = a.H * (kHeadDim / 8);
+      for (int i = tid; i < r.ql * chunks; i += 128)
+        reinterpret_cast<uint4*>(a.out + (long long)(r.q_start + i / chunks) * a.out_row_stride)[i % chunks] =
+            make_uint4(0u, 0u, 0u, 0u);
+    }
+  } else if (ntiles > 0) {
+    // ------------------------------------------------------------------ softmax / correction / epilogue
+    const int wg = (warp - 4) >> 2;          // column group: columns cb .. cb + 15
+    const int cb = wg * 16;
+    const int w = warp & 3;                  // TMEM lane quadrant
+    const int row = (threadIdx.x - 128) & 127;   // key within the tile (S^T) / head dim (O^T)
+    const int col = cb + (lane & 15);
+    const uint32_t lane_off = static_cast<uint32_t>(w * 32) << 16;
+    const int bar_wg = 1 + wg;
+    const long long T = S.total_tiles, Ge = S.active;
+    const int c = blockIdx.x;
+    const int my_group = row / a.group;
+    Walk<QMAX, true> wk;
+    wk.start(a, S);
+    bool ok = true;
+    int g = 0;
+    for (int n = 0; ok && wk.A < x_end; wk.next(a), ++n) {
+      const int L = wk.r.L, ql = wk.r.ql;
+      const int t0 = wk.t0(x_begin), t1 = wk.t1(x_end);
+      const uint32_t tmem_o = tmem + lane_off + kTmemO + (n & 1) * kTmemOStride + cb;
+      const int min_limit = a.causal ? L - ql : L - 1;       // smallest limit among the valid columns
+      const long long c_lo = ceil_div((wk.A + 1) * Ge, T) - 1, c_hi = ceil_div((wk.A + wk.r.nt) * Ge, T) - 1;
+      int seen_early = -1;
+      if (threadIdx.x == 128 && c_lo != c_hi && c == c_lo)
+        seen_early = ld_acquire_gpu(a.counters + (long long)wk.b * a.Hkv + wk.h);
+      float q_factor = 0.0f;
+      // running maxima of t (log2 domain; lane j owns column cb + (j & 15)'s), every thread's copy less the bias, and
+      // this thread's share of the column sums
+      float m_lane = kNegBig, m_all[16], l_part[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        m_all[j] = kNegBig;
+        l_part[j] = 0.0f;
+      }
+      for (int t = t0; t < t1; ++t, ++g) {
+        const int buf = g & 1;
+        const int e = g % kScaleStages;
+        if (!mbar_wait(&S.sc_full[e], (g / kScaleStages) & 1, abort, a.err, kErrTimeoutScale)) { ok = false; break; }
+        const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.sc_empty[e]);
+        const float log_vs = __log2f(vs), inv_vs = 1.0f / vs;
+        if (!mbar_wait(&S.s_full[buf], (g >> 1) & 1, abort, a.err, kErrTimeoutS)) { ok = false; break; }
+        tc_fence_after();
+        if (t == t0) q_factor = S.q_scale[n & 3] * a.scale_log2;
+        float x[16], x2[16];
+        tmem_ld_32x32b_x16(tmem + lane_off + buf * 64 + cb, x);
+        tmem_ld_32x32b_x16(tmem + lane_off + buf * 64 + 32 + cb, x2);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.s_free[buf]);
+        const float factor = ks * q_factor;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = fmaf(fmaf(x2[j], 0.0625f, x[j]), factor, log_vs);
+        const int key = t * kKeysPerTile + row;
+        if ((t * kKeysPerTile + kKeysPerTile - 1) > min_limit) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int p = (cb + j) / G;
+            const int limit = (a.causal && p < ql) ? L - ql + p : L - 1;
+            x[j] = key <= limit ? x[j] : -INFINITY;
+          }
+        }
+        // ---- column maxima: this warp's (lane j keeps column cb + j's), then the four warps'
+        float wmax = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float v = warp_max_redux(x[j]);
+          wmax = lane == j ? v : wmax;
+        }
+        if (lane < 16) S.red_max[buf][col][w] = wmax;
+        named_barrier(bar_wg, 128);
+        const float4 r4 = *reinterpret_cast<const float4*>(S.red_max[buf][col]);
+        const float tmax = fmaxf(fmaxf(r4.x, r4.y), fmaxf(r4.z, r4.w));
+        const bool grow = tmax > m_lane + 8.0f;
+        if (__any_sync(0xffffffffu, grow)) {       // uniform over the group's 128 threads
+          const float m_new = grow ? tmax : m_lane;
+          const float alpha_lane = ex2_approx(m_lane - m_new);
+          m_lane = m_new;
+          float alpha[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            alpha[j] = __shfl_sync(0xffffffffu, alpha_lane, j);
+            m_all[j] = __shfl_sync(0xffffffffu, m_new, j) - kPBias;
+            l_part[j] *= alpha[j];
+          }
+          if (t > t0) {     // O holds this item's earlier tiles: rescale its parts once PV(g-1) has landed
+            if (!mbar_wait(&S.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int part = 0; part < kPParts; ++part) {
+              float o[16];
+              tmem_ld_32x32b_x16(tmem_o + part * kCols, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] *= alpha[j];
+              tmem_st_32x32b_x16(tmem_o + part * kCols, o);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          x[j] = ex2_approx(x[j] - m_all[j]);      // masked: 0
+          l_part[j] = fmaf(x[j], inv_vs, l_part[j]);
+        }
+        // ---- this group's 16 columns of row `row` of the three parts, once PV(g-2) released the buffer
+        if (g >= 2 && !mbar_wait(&S.o_done[buf], ((g - 2) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
+        unsigned char* prow = sP + buf * kPBytes + row * kCols + (wg ^ ((row >> 2) & 1)) * 16;
+#pragma unroll
+        for (int part = 0; part < kPParts; ++part) {
+          unsigned wd[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = x[4 * k + i];
+              y[i] = part < kPParts - 1 ? cut3(v) : v;
+              x[4 * k + i] = v - y[i];
+            }
+            wd[k] = encode_e5m2x2(y[0], y[1]) | encode_e5m2x2(y[2], y[3]) << 16;
+          }
+          *reinterpret_cast<uint4*>(prow + part * kPPartBytes) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+        }
+        // ---- the row's last tile: V rows past the context are zeroed; each group zeroes half of the row
+        if ((t + 1) * kKeysPerTile > L) {
+          const int stage = g % kStages;
+          if (!mbar_wait(&S.v_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutV)) { ok = false; break; }
+          if (key >= L) {
+            unsigned char* v0 = sV + stage * kTileBytes + row * kHeadDim + wg * 64;
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) *reinterpret_cast<uint4*>(v0 + cc * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.p_full[buf]);
+      }
+      if (!ok) break;
+      // ---- item epilogue: column sums over the 128 key threads, O^T out of TMEM
+      {
+        const float s = column_reduce16(l_part, lane);
+        if (lane < 16) S.red_sum[col][w] = s;
+      }
+      named_barrier(bar_wg, 128);
+      const int gl = g - 1;
+      if (!mbar_wait(&S.o_done[gl & 1], (gl >> 1) & 1, abort, a.err, kErrTimeoutO)) break;
+      tc_fence_after();
+      float o[16];
+      tmem_ld_32x32b_x16(tmem_o, o);
+#pragma unroll
+      for (int part = 1; part < kPParts; ++part) {
+        float o2[16];
+        tmem_ld_32x32b_x16(tmem_o + part * kCols, o2);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] += o2[j];
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.o_free[n & 1]);
+      const float4 s4 = *reinterpret_cast<const float4*>(S.red_sum[col]);
+      float l_lane = (s4.x + s4.y) + (s4.z + s4.w);
+      // ---- a split item: pieces published, the last to arrive merges them in CTA order (as the bf16 kernel)
+      const long long A = wk.A;
+      if (c_lo != c_hi) {
+        int* counter = a.counters + (long long)wk.b * a.Hkv + wk.h;
+        if (threadIdx.x == 128) {
+          const int need = (int)(c_hi - c_lo);
+          S.last_piece = (c == c_lo && (seen_early == need || ld_acquire_gpu(counter) == need)) ? 2 : 0;
+        }
+        named_barrier(3, 256);
+        const bool own_in_registers = S.last_piece == 2;
+        if (!own_in_registers) {
+          float* mine = a.partial + (2LL * c + (x_begin < A ? 1 : 0)) * kPartialFloats;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) __stcg(mine + (cb + j) * kHeadDim + row, o[j]);
+          if (w == 0 && lane < 16) {
+            __stcg(mine + kCols * kHeadDim + col, m_lane);
+            __stcg(mine + kCols * kHeadDim + kCols + col, l_lane);
+          }
+          __threadfence();
+          named_barrier(3, 256);
+          if (threadIdx.x == 128) {
+            const int last = atomicAdd(counter, 1) == (int)(c_hi - c_lo);
+            if (last) atomicExch(counter, 0);
+            S.last_piece = last;
+          }
+          named_barrier(3, 256);
+          if (!S.last_piece) continue;
+        } else if (threadIdx.x == 128) {
+          atomicExch(counter, 0);
+        }
+        __threadfence();
+        float m_acc = kNegBig, l_acc = 0.0f;
+        const float m_own = m_lane, l_own = l_lane;
+        auto merge = [&](float mp, float lp, const float* op) {
+          const float mn = fmaxf(m_acc, mp);
+          const float sa = ex2_approx(m_acc - mn), sb = ex2_approx(mp - mn);
+          m_acc = mn;
+          l_acc = __fmaf_rn(lp, sb, __fmul_rn(l_acc, sa));
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            o[j] = __fmaf_rn(op ? __ldcg(op + (cb + j) * kHeadDim + row) : o[j], __shfl_sync(0xffffffffu, sb, j),
+                             __fmul_rn(op ? o[j] : 0.0f, __shfl_sync(0xffffffffu, sa, j)));
+        };
+        long long cc = c_lo;
+        if (own_in_registers) {
+          merge(m_own, l_own, nullptr);
+          ++cc;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+        }
+        for (; cc <= c_hi; ++cc) {
+          const long long s_cc = T * cc / Ge;
+          const float* piece = a.partial + (2 * cc + (s_cc < A ? 1 : 0)) * kPartialFloats;
+          merge(__ldcg(piece + kCols * kHeadDim + col), __ldcg(piece + kCols * kHeadDim + kCols + col), piece);
+        }
+        l_lane = l_acc;
+      }
+      const float inv_lane = l_lane > 0.0f ? 1.0f / l_lane : l_lane;      // nothing seen: 0 (and NaN stays)
+      const int d = row;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int p = (cb + j) / G, gq = (cb + j) % G;
+        const float inv = __shfl_sync(0xffffffffu, inv_lane, j);
+        if (p < ql)
+          a.out[(long long)(wk.r.q_start + p) * a.out_row_stride + (long long)(wk.h * G + gq) * kHeadDim + d] =
+              __float2bfloat16_rn(o[j] * inv);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// 3-D map of a code cache: {128 dims, block_size slots, blocks * heads}, 128-byte swizzle, box {128, keys, 1}.
+static int make_map(CUtensorMap* map, const void* base, uint64_t block_size, uint64_t block_heads, uint32_t keys) {
+  auto fn = encoder();
+  if (!fn) return set_error(kCudaError, "cuTensorMapEncodeTiled is unavailable from the driver");
+  cuuint64_t dims[3] = {kHeadDim, block_size, block_heads};
+  cuuint64_t strides[2] = {kHeadDim, kHeadDim * block_size};
+  cuuint32_t box[3] = {kHeadDim, keys, 1};
+  cuuint32_t elem[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(kCudaError, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return kOk;
+}
+
+template <int G>
+static int launch(const CUtensorMap (&m)[4], const Args& a, int grid, bool early, cudaStream_t stream) {
+  if (int st = ensure_dynamic_smem<verify_attention_fp8_kernel<G>>(kSmemBytes)) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  SPECDEC_CUDA_TRY(cudaLaunchKernelEx(&cfg, verify_attention_fp8_kernel<G>, m[0], m[1], m[2], m[3], a));
+  SPECDEC_LAUNCH_CHECK();
+  return kOk;
 }
 
 }  // namespace attention_fp8
@@ -114,6 +701,7 @@ int specdec_paged_attention_fp8(const void* q, long long T, long long q_row_stri
                     "unknown flags 0x%x", flags);
   SPECDEC_CHECK_ARG(q && k_cache && v_cache && k_scale && v_scale && block_tables && out && workspace && err,
                     "null pointer argument");
+  SPECDEC_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "workspace must be 256-byte aligned");
   SPECDEC_CHECK_ARG(head_dim == kHeadDim, "head_dim %d: this build implements 128", head_dim);
   SPECDEC_CHECK_ARG(num_kv_heads >= 1 && num_heads >= 1 && num_heads % num_kv_heads == 0,
                     "heads %d not a multiple of kv heads %d", num_heads, num_kv_heads);
@@ -126,28 +714,65 @@ int specdec_paged_attention_fp8(const void* q, long long T, long long q_row_stri
   SPECDEC_CHECK_ARG(block_size >= 1 && block_size % kKeysPerTile == 0, "block_size %d must be a multiple of %d",
                     block_size, kKeysPerTile);
   SPECDEC_CHECK_ARG(scale_group == 16 || scale_group == 32, "scale_group %d: 16 or 32 slots share a scale", scale_group);
-  SPECDEC_CHECK_ARG(R >= 1 && R <= 65535 && W >= 1 && T >= 1, "bad row/table sizes");
+  SPECDEC_CHECK_ARG(R >= 1 && R <= 65535 && W >= 1 && T >= 1 && T <= 0x7fffffffLL, "bad row/table sizes");
   SPECDEC_CHECK_ARG((cu_seqlens_q && cu_seqlens_k) || (context_lens && q_per_seq >= 1),
                     "give cu_seqlens_q/k (varlen) or context_lens and q_per_seq (decode)");
   SPECDEC_CHECK_ARG(cu_seqlens_q || (q_per_seq <= max_seqlen_q && (long long)R * q_per_seq <= T),
                     "decode mode: q_per_seq must fit the batch");
   SPECDEC_CHECK_ARG(num_blocks >= 1 && num_blocks <= 0x7fffffffLL / num_kv_heads, "num_blocks * kv heads must fit 32 bits");
-  SPECDEC_CHECK_ARG((long long)W * block_size <= 0x7fffffffLL, "a row's table spans more than 2^31 keys");
+  SPECDEC_CHECK_ARG((long long)W * block_size <= 0x7fffffffLL - kKeysPerTile, "a row's table spans more than 2^31 keys");
   SPECDEC_CHECK_ARG((reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_row_stride % 8 == 0 && out_row_stride % 8 == 0 &&
                         (reinterpret_cast<uintptr_t>(out) & 15) == 0,
                     "q and out rows must be 16-byte aligned");
   SPECDEC_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
                       reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 15) == 0,
                     "caches and scales must be 16-byte aligned");
-  Args a{static_cast<const __nv_bfloat16*>(q), q_row_stride, static_cast<const unsigned char*>(k_cache),
-         static_cast<const unsigned char*>(v_cache), k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, context_lens,
-         q_per_seq, R, max_seqlen_q, block_tables, W, block_size, scale_group, num_blocks, num_heads, num_kv_heads,
-         softmax_scale, causal, static_cast<__nv_bfloat16*>(out), out_row_stride, err};
-  const int warps = max_seqlen_q * num_heads;
-  dim3 grid((unsigned)R, (unsigned)((warps + 7) / 8));
-  simple_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  SPECDEC_LAUNCH_CHECK();
-  return kOk;
+  DeviceInfo info;
+  if (int st = device_info(&info)) return st;
+  const long long need = attention::workspace_bytes(R, num_kv_heads, info.sm_count);
+  if (workspace_bytes < need)
+    return set_error(kWorkspaceTooSmall, "attention workspace of %lld bytes, %lld needed", workspace_bytes, need);
+  CUtensorMap m[4];
+  const uint64_t bh = (uint64_t)num_blocks * num_kv_heads;
+  for (int i = 0; i < 4; ++i)
+    if (int st = make_map(&m[i], i & 1 ? v_cache : k_cache, block_size, bh, i < 2 ? kKeysPerTile : kSubKeys)) return st;
+  Args a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_row_stride = q_row_stride;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.cu_seqlens_q = cu_seqlens_q;
+  a.cu_seqlens_k = cu_seqlens_k;
+  a.context_lens = context_lens;
+  a.q_per_seq = q_per_seq;
+  a.R = R;
+  a.T = (int)T;
+  a.block_tables = block_tables;
+  a.W = W;
+  a.block_size = block_size;
+  a.group = scale_group;
+  a.num_blocks = (int)num_blocks;
+  a.H = num_heads;
+  a.Hkv = num_kv_heads;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.causal = causal;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.out_row_stride = out_row_stride;
+  a.err = err;
+  a.partial = static_cast<float*>(workspace);
+  a.counters = reinterpret_cast<int*>(static_cast<unsigned char*>(workspace) + partial_bytes(info.sm_count));
+  const long long max_tiles = (long long)R * num_kv_heads * ((long long)W * block_size / kKeysPerTile);
+  const int cap = (int)((flags >> SPECDEC_ATTN_CTAS_SHIFT) & 0xffu);
+  const int ctas = cap > 0 && cap < info.sm_count ? cap : info.sm_count;
+  const int grid = (int)(max_tiles < ctas ? max_tiles : ctas);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool early = (flags & SPECDEC_ATTN_EARLY_LAUNCH) != 0;
+  switch (G) {
+    case 1: return launch<1>(m, a, grid, early, s);
+    case 2: return launch<2>(m, a, grid, early, s);
+    case 4: return launch<4>(m, a, grid, early, s);
+    default: return launch<8>(m, a, grid, early, s);
+  }
 }
 
 }  // extern "C"

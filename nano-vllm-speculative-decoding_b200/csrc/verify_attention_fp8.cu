@@ -450,13 +450,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.sc_empty[e]);
-        const float log_vs = __log2f(vs), inv_vs = 1.0f / vs;
+        const float log_vs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
         if (!mbar_wait(&S.s_full[buf], (g >> 1) & 1, abort, a.err, kErrTimeoutS)) { ok = false; break; }
         tc_fence_after();
         if (t == t0) q_factor = S.q_scale[n & 3] * a.scale_log2;
         float x[16], x2[16];
-        tmem_ld_32x32b_x16(tmem + lane_off + buf * 64 + cb, x);
-        tmem_ld_32x32b_x16(tmem + lane_off + buf * 64 + 32 + cb, x2);
+        tmem_ld_32x32b_2x16(tmem + lane_off + buf * 64 + cb, tmem + lane_off + buf * 64 + 32 + cb, x, x2);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.s_free[buf]);
@@ -472,20 +471,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             x[j] = key <= limit ? x[j] : -INFINITY;
           }
         }
-        // ---- column maxima: this warp's (lane j keeps column cb + j's), then the four warps'
-        float wmax = -INFINITY;
+        // ---- does any score of the group pass its column's running maximum by more than 2^8?  Only then (always at an
+        // item's first tile) are the tile's column maxima taken: this warp's, then the four warps'
+        float over = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float v = warp_max_redux(x[j]);
-          wmax = lane == j ? v : wmax;
-        }
-        if (lane < 16) S.red_max[buf][col][w] = wmax;
-        named_barrier(bar_wg, 128);
-        const float4 r4 = *reinterpret_cast<const float4*>(S.red_max[buf][col]);
-        const float tmax = fmaxf(fmaxf(r4.x, r4.y), fmaxf(r4.z, r4.w));
-        const bool grow = tmax > m_lane + 8.0f;
-        if (__any_sync(0xffffffffu, grow)) {       // uniform over the group's 128 threads
-          const float m_new = grow ? tmax : m_lane;
+        for (int j = 0; j < 16; ++j) over = fmaxf(over, x[j] - m_all[j]);
+        if (named_barrier_or(bar_wg, 128, over > 8.0f + kPBias)) {
+          float wmax = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float v = warp_max_redux(x[j]);
+            wmax = lane == j ? v : wmax;
+          }
+          if (lane < 16) S.red_max[buf][col][w] = wmax;
+          named_barrier(bar_wg, 128);
+          const float4 r4 = *reinterpret_cast<const float4*>(S.red_max[buf][col]);
+          const float tmax = fmaxf(fmaxf(r4.x, r4.y), fmaxf(r4.z, r4.w));
+          const float m_new = tmax > m_lane + 8.0f ? tmax : m_lane;
           const float alpha_lane = ex2_approx(m_lane - m_new);
           m_lane = m_new;
           float alpha[16];

@@ -24,9 +24,9 @@
 // The scales never touch the codes: ks_j multiplies the score, and vs_j goes into the exponent: with t_j = s_j + log2 vs_j
 // the running maximum is over t, the tensor core gets p'_j = 2^(t_j - m) (so the largest contribution keeps every bit
 // whatever the scales' spread), and the denominator sums p'_j / vs_j.
-//   warp 0       TMA producer: the K tiles             warps 4-11   softmax over keys (a TMEM lane is a key; two groups of
-//   warp 1       TMEM allocator, MMA issuer                          16 columns each), P parts, O rescale, epilogue
-//   warp 2       prologue; producer of the scales      warps 12-15  query parts of the next items; rows without keys
+//   warp 0       TMA producer: K tiles and the scales  warps 4-19   softmax over keys (a TMEM lane is a key; four groups of
+//   warp 1       TMEM allocator, MMA issuer                          8 columns each), P parts, O rescale, epilogue
+//   warp 2       prologue                              warps 20-23  query parts of the next items; rows without keys
 //   warp 3       TMA producer: the V tiles
 // Softmax: online per column with lazy rescaling (O is rescaled when a column's maximum grows by more than 2^8; p' reaches
 // 2^15 then, in e5m2's range), masked by key index.  V rows past the context are zeroed in shared memory.
@@ -43,8 +43,15 @@ using namespace attention;
 
 constexpr int kSubKeys = 32;                          // an item's last tile loads in 32-key sub-boxes
 constexpr int kStages = 5;                            // K ring and V ring depth: 160 KB in flight
-constexpr int kScaleStages = 8;                       // scale ring depth
-constexpr int kThreads = 512;
+// Scale ring depth.  A tile's scales arrive on its K tile's barrier.  The entry of tile g is written again for tile
+// g + 8, which K's producer reaches after S(g + 3) is done; S(g + 3) goes out after the softmax has handed over P(g + 1).
+constexpr int kScaleStages = 8;
+static_assert(kScaleStages >= kStages + 2, "a scale entry must outlive the softmax's reads");
+constexpr int kGroups = 4, kGroupCols = kCols / kGroups;   // softmax warpgroups, 8 columns each
+constexpr int kSoftmaxWarp = 4, kSoftmaxThreads = kGroups * 128, kSoftmaxWarps = kSoftmaxThreads / 32;
+constexpr int kQueryWarp = kSoftmaxWarp + kSoftmaxWarps;
+constexpr int kThreads = kQueryWarp * 32 + 128;
+constexpr int kBarMerge = 1 + kGroups, kBarQuery = 2 + kGroups;   // named barriers: 1 .. kGroups are the groups'
 constexpr int kTileBytes = kKeysPerTile * kHeadDim;   // 16 KB of codes
 constexpr int kQParts = 2, kPParts = 3;
 constexpr int kQBytes = kQParts * kCols * kHeadDim;   // 8 KB, double-buffered by item
@@ -56,7 +63,7 @@ constexpr float kPBias = 7.0f;                        // p' is kept 2^7 up: its 
 constexpr float kMinScale = 7.888609052210118e-31f;   // 2^-100, the store's smallest scale
 
 constexpr int kErrTimeoutQ = 11, kErrTimeoutK = 12, kErrTimeoutV = 13, kErrTimeoutS = 14, kErrTimeoutP = 15,
-              kErrTimeoutO = 16, kErrTimeoutEmpty = 17, kErrTimeoutScale = 18, kErrPage = 5;
+              kErrTimeoutO = 16, kErrTimeoutEmpty = 17, kErrPage = 5;
 
 struct Args {
   const __nv_bfloat16* q;    // [T, H, D]
@@ -82,8 +89,7 @@ struct Args {
 struct Smem {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t sc_full[kScaleStages], sc_empty[kScaleStages];
-  uint64_t s_full[2], s_free[2], p_full[2], o_done[2], o_free[2];
+  uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
   alignas(16) float scales[kScaleStages][2][kKeysPerTile / 16];   // [ring][K, V][group of the tile]
   alignas(16) float red_max[2][32][4];   // [tile parity][column][warp] maxima
   alignas(16) float red_sum[32][4];
@@ -148,20 +154,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&S.q_full[i], 4);     // one elected arrival per query warp
       mbar_init(&S.q_empty[i], 1);
       mbar_init(&S.s_full[i], 1);
-      mbar_init(&S.s_free[i], 8);     // one per softmax warp
-      mbar_init(&S.p_full[i], 8);
+      mbar_init(&S.p_full[i], kSoftmaxWarps);     // one elected arrival per softmax warp
       mbar_init(&S.o_done[i], 1);
-      mbar_init(&S.o_free[i], 8);
+      mbar_init(&S.o_free[i], kSoftmaxWarps);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&S.k_full[s], 1);
       mbar_init(&S.k_empty[s], 1);
       mbar_init(&S.v_full[s], 1);
       mbar_init(&S.v_empty[s], 1);
-    }
-    for (int s = 0; s < kScaleStages; ++s) {
-      mbar_init(&S.sc_full[s], 1);
-      mbar_init(&S.sc_empty[s], 8);
     }
     S.abort = 0;
     fence_barrier_init();
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int ntiles = (int)(x_end - x_begin);
 
   if (warp == 0 || warp == 3) {
-    // ------------------------------------------------------------------ TMA producers of the codes
+    // ------------------------------------------------------------------ TMA producers: K with both scales, V
     const bool is_k = warp == 0;
     if (lane == 0 && ntiles > 0) {
       uint64_t* full = is_k ? S.k_full : S.v_full;
@@ -219,6 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       unsigned char* ring = is_k ? sK : sV;
       const CUtensorMap* map = is_k ? &kmap : &vmap;
       const CUtensorMap* map32 = is_k ? &kmap32 : &vmap32;
+      const int per_tile = kKeysPerTile / a.group, per_block = a.block_size / a.group;
+      const uint32_t scale_bytes = per_tile * 4;
       Walk<QMAX, true> wk;
       wk.start(a, S);
       bool ok = true;
@@ -238,109 +241,92 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int subs = t == wk.r.nt - 1 ? (wk.r.L - key0 + kSubKeys - 1) / kSubKeys : kKeysPerTile / kSubKeys;
           unsigned char* dst = ring + stage * kTileBytes;
-          mbar_arrive_expect_tx(&full[stage], subs * kSubKeys * kHeadDim);
+          mbar_arrive_expect_tx(&full[stage], subs * kSubKeys * kHeadDim + (is_k ? 2 * scale_bytes : 0));
           if (subs == kKeysPerTile / kSubKeys) {
             tma_load_3d(dst, map, 0, j0, ph, &full[stage]);
           } else {
             for (int j = 0; j < subs; ++j)
               tma_load_3d(dst + j * kSubKeys * kHeadDim, map32, 0, j0 + j * kSubKeys, ph, &full[stage]);
           }
-        }
-      }
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------------ producer of the scales
-    if (lane == 0 && ntiles > 0) {
-      const int per_tile = kKeysPerTile / a.group, per_block = a.block_size / a.group;
-      const uint32_t bytes = per_tile * 4;
-      Walk<QMAX, true> wk;
-      wk.start(a, S);
-      bool ok = true;
-      int g = 0;
-      for (; ok && wk.A < x_end; wk.next(a)) {
-        const int* table = a.block_tables + (long long)wk.b * a.W;
-        const int t1 = wk.t1(x_end);
-        for (int t = wk.t0(x_begin); t < t1; ++t, ++g) {
-          const int e = g % kScaleStages;
-          const int key0 = t * kKeysPerTile;
-          const int page = g == 0 ? S.page0 : page_of(a, table, key0);
-          const long long at =
-              ((long long)page * a.Hkv + wk.h) * per_block + key0 % a.block_size / kKeysPerTile * per_tile;
-          if (g >= kScaleStages &&
-              !mbar_wait(&S.sc_empty[e], (g / kScaleStages - 1) & 1, abort, a.err, kErrTimeoutEmpty)) {
-            ok = false;
-            break;
+          if (is_k) {
+            const long long at = (long long)ph * per_block + j0 / kKeysPerTile * per_tile;
+            bulk_load(S.scales[g % kScaleStages][0], a.k_scale + at, scale_bytes, &full[stage]);
+            bulk_load(S.scales[g % kScaleStages][1], a.v_scale + at, scale_bytes, &full[stage]);
           }
-          mbar_arrive_expect_tx(&S.sc_full[e], 2 * bytes);
-          bulk_load(S.scales[e][0], a.k_scale + at, bytes, &S.sc_full[e]);
-          bulk_load(S.scales[e][1], a.v_scale + at, bytes, &S.sc_full[e]);
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0 && ntiles > 0) {
-      const uint32_t idesc_s = idesc_f8_f32(128, kQParts * kCols, 0, 0, 0, 0);    // e4m3 . e4m3
-      const uint32_t idesc_o = idesc_f8_f32(128, kPParts * kCols, 0, 1, 1, 1);    // e4m3 . e5m2
+      constexpr uint32_t idesc_s = idesc_f8_f32(128, kQParts * kCols, 0, 0, 0, 0);    // e4m3 . e4m3
+      constexpr uint32_t idesc_o = idesc_f8_f32(128, kPParts * kCols, 0, 1, 1, 1);    // e4m3 . e5m2
+      // descriptors of the first buffers; the others differ in the low word's address (16-byte units)
+      const uint64_t kd = smem_desc(sK, 16, 1024, kSwizzle128B), qd = smem_desc(sQ, 16, 1024, kSwizzle128B);
+      const uint64_t vd = smem_desc(sV, kTileBytes, 1024, kSwizzle128B), pd = smem_desc(sP, kPPartBytes, 256, kSwizzle32B);
+      const uint32_t kd_hi = (uint32_t)(kd >> 32), qd_hi = (uint32_t)(qd >> 32), vd_hi = (uint32_t)(vd >> 32),
+                     pd_hi = (uint32_t)(pd >> 32);
       Cursor<QMAX, true> cs, cp;     // the score MMAs run two tiles ahead of the PV MMAs
       cs.start(a, S);
       cp.start(a, S);
+      int sk = 0, sv = 0;            // ring stages of the next K and V tile, and their phases
+      uint32_t sk_phase = 0, sv_phase = 0;
       auto issue_s = [&](int g) -> bool {
-        const int stage = g % kStages;
         const int qb = cs.n & 1;
         if (cs.first && !mbar_wait(&S.q_full[qb], (cs.n >> 1) & 1, abort, a.err, kErrTimeoutQ)) return false;
-        if (!mbar_wait(&S.k_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutK)) return false;
-        if (g >= 2 && !mbar_wait(&S.s_free[g & 1], ((g - 2) >> 1) & 1, abort, a.err, kErrTimeoutS)) return false;
+        if (!mbar_wait(&S.k_full[sk], sk_phase, abort, a.err, kErrTimeoutK)) return false;
         tc_fence_after();
-        const unsigned char* kt = sK + stage * kTileBytes;
-        const unsigned char* qt = sQ + qb * kQBytes;
+        const uint32_t ka = (uint32_t)kd + sk * (kTileBytes >> 4), qa = (uint32_t)qd + qb * (kQBytes >> 4);
         const uint32_t tmem_s = tmem + (g & 1) * 64;
 #pragma unroll
-        for (int kk = 0; kk < kHeadDim / 32; ++kk) {
-          const uint64_t adesc = smem_desc(kt + kk * 32, 16, 1024, kSwizzle128B);
-          const uint64_t bdesc = smem_desc(qt + kk * 32, 16, 1024, kSwizzle128B);
-          mma_f8_ss(tmem_s, adesc, bdesc, idesc_s, kk > 0 ? 1u : 0u);
-        }
+        for (int kk = 0; kk < kHeadDim / 32; ++kk)
+          mma_f8_ss(tmem_s, ka + kk * 2, kd_hi, qa + kk * 2, qd_hi, idesc_s, kk > 0 ? 1u : 0u);
         mma_commit(&S.s_full[g & 1]);
-        mma_commit(&S.k_empty[stage]);
+        mma_commit(&S.k_empty[sk]);
         if (cs.last()) mma_commit(&S.q_empty[qb]);
+        if (++sk == kStages) {
+          sk = 0;
+          sk_phase ^= 1;
+        }
         cs.advance(a, x_begin, x_end);
         return true;
       };
       auto issue_pv = [&](int g) -> bool {
-        const int stage = g % kStages;
         const int ob = cp.n & 1;
         if (cp.first && cp.n >= 2 && !mbar_wait(&S.o_free[ob], ((cp.n - 2) >> 1) & 1, abort, a.err, kErrTimeoutO))
           return false;
+        if (!mbar_wait(&S.v_full[sv], sv_phase, abort, a.err, kErrTimeoutV)) return false;
         if (!mbar_wait(&S.p_full[g & 1], (g >> 1) & 1, abort, a.err, kErrTimeoutP)) return false;
-        if (!mbar_wait(&S.v_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutV)) return false;
         tc_fence_after();
-        const unsigned char* vt = sV + stage * kTileBytes;
-        const unsigned char* pt = sP + (g & 1) * kPBytes;
+        const uint32_t va = (uint32_t)vd + sv * (kTileBytes >> 4), pa = (uint32_t)pd + (g & 1) * (kPBytes >> 4);
         const uint32_t tmem_o = tmem + kTmemO + ob * kTmemOStride;
-        const bool fresh = cp.first;
+        const uint32_t fresh = cp.first ? 0u : 1u;
 #pragma unroll
-        for (int kk = 0; kk < kKeysPerTile / 32; ++kk) {
-          const uint64_t adesc = smem_desc(vt + kk * 32 * kHeadDim, kTileBytes, 1024, kSwizzle128B);
-          const uint64_t bdesc = smem_desc(pt + kk * 32 * kCols, kPPartBytes, 256, kSwizzle32B);
-          mma_f8_ss(tmem_o, adesc, bdesc, idesc_o, (!fresh || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < kKeysPerTile / 32; ++kk)
+          mma_f8_ss(tmem_o, va + kk * (32 * kHeadDim >> 4), vd_hi, pa + kk * (32 * kCols >> 4), pd_hi, idesc_o,
+                    kk > 0 ? 1u : fresh);
         mma_commit(&S.o_done[g & 1]);
-        mma_commit(&S.v_empty[stage]);
+        mma_commit(&S.v_empty[sv]);
+        if (++sv == kStages) {
+          sv = 0;
+          sv_phase ^= 1;
+        }
         cp.advance(a, x_begin, x_end);
         return true;
       };
+      // PV(g) goes out before S(g + 2).  The wait for P(g) says that the softmax has read S(g) and the tile's scales, so
+      // S's buffer is free; and as MMAs complete in order, a softmax that sees S(g + 2) knows that PV(g) has read P's.
       bool ok = issue_s(0);
       if (ok && ntiles > 1) ok = issue_s(1);
       for (int g = 0; g < ntiles && ok; ++g) {
-        if (g + 2 < ntiles) ok = issue_s(g + 2);
-        if (ok) ok = issue_pv(g);
+        ok = issue_pv(g);
+        if (ok && g + 2 < ntiles) ok = issue_s(g + 2);
       }
     }
-  } else if (warp >= 12) {
+  } else if (warp >= kQueryWarp) {
     // ------------------------------------------------------------------ query parts: 32 columns x 128 dims an item
     // a column's 128 dims belong to four threads, 32 each
-    const int tid = threadIdx.x - 384, col = tid >> 2, quarter = tid & 3;
+    const int tid = threadIdx.x - kQueryWarp * 32, col = tid >> 2, quarter = tid & 3;
     const int p = col / G, gq = col % G;
     if (ntiles > 0) {
       Walk<QMAX, true> wk;
@@ -362,9 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         most = __reduce_max_sync(0xffffffffu, most);
-        named_barrier(4, 128);                 // the last item's maxima have been read
-        if (lane == 0) S.red_q[warp - 12] = most;
-        named_barrier(4, 128);
+        named_barrier(kBarQuery, 128);         // the last item's maxima have been read
+        if (lane == 0) S.red_q[warp - kQueryWarp] = most;
+        named_barrier(kBarQuery, 128);
         most = max(max(S.red_q[0], S.red_q[1]), max(S.red_q[2], S.red_q[3]));
         // 2^e with every |q| <= 448 * 2^e = 1.75 * 2^(e + 8)
         int e = (int)(most >> 7) - 135 + ((most & 0x7fu) > 0x60u ? 1 : 0);
@@ -393,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(q2 + phys) = make_uint4(b2[0] | b2[1] << 16, b2[2] | b2[3] << 16,
                                                             b2[4] | b2[5] << 16, b2[6] | b2[7] << 16);
         }
-        // read by the softmax before it frees the item's first score tile; written again four items on, after that
+        // read by the softmax before it hands over P of the item's first tile; written again four items on, after that
         if (tid == 0) S.q_scale[n & 3] = __uint_as_float((unsigned)(e + 127) << 23);
         fence_proxy_async_smem();
         __syncwarp();
@@ -409,15 +395,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         reinterpret_cast<uint4*>(a.out + (long long)(r.q_start + i / chunks) * a.out_row_stride)[i % chunks] =
             make_uint4(0u, 0u, 0u, 0u);
     }
-  } else if (ntiles > 0) {
+  } else if (warp >= kSoftmaxWarp && ntiles > 0) {
     // ------------------------------------------------------------------ softmax / correction / epilogue
-    const int wg = (warp - 4) >> 2;          // column group: columns cb .. cb + 15
-    const int cb = wg * 16;
-    const int w = warp & 3;                  // TMEM lane quadrant
-    const int row = (threadIdx.x - 128) & 127;   // key within the tile (S^T) / head dim (O^T)
-    const int col = cb + (lane & 15);
+    const int wg = (warp - kSoftmaxWarp) >> 2;   // column group: columns cb .. cb + 7
+    const int cb = wg * kGroupCols;
+    const int w = warp & 3;                      // TMEM lane quadrant
+    const int row = (threadIdx.x - kSoftmaxWarp * 32) & 127;   // key within the tile (S^T) / head dim (O^T)
+    const int col = cb + (lane & 7);             // the column that lane j (and j + 8, ..) speaks for
     const uint32_t lane_off = static_cast<uint32_t>(w * 32) << 16;
     const int bar_wg = 1 + wg;
+    const bool first_thread = threadIdx.x == kSoftmaxWarp * 32;
     const long long T = S.total_tiles, Ge = S.active;
     const int c = blockIdx.x;
     const int my_group = row / a.group;
@@ -430,118 +417,121 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t0 = wk.t0(x_begin), t1 = wk.t1(x_end);
       const uint32_t tmem_o = tmem + lane_off + kTmemO + (n & 1) * kTmemOStride + cb;
       const int min_limit = a.causal ? L - ql : L - 1;       // smallest limit among the valid columns
+      // A group none of whose columns holds a query only keeps the barriers going: its columns of P and O are never read.
+      const bool live = cb < ql * G;
       const long long c_lo = ceil_div((wk.A + 1) * Ge, T) - 1, c_hi = ceil_div((wk.A + wk.r.nt) * Ge, T) - 1;
       int seen_early = -1;
-      if (threadIdx.x == 128 && c_lo != c_hi && c == c_lo)
+      if (first_thread && c_lo != c_hi && c == c_lo)
         seen_early = ld_acquire_gpu(a.counters + (long long)wk.b * a.Hkv + wk.h);
       float q_factor = 0.0f;
-      // running maxima of t (log2 domain; lane j owns column cb + (j & 15)'s), every thread's copy less the bias, and
+      // running maxima of t (log2 domain; lane j owns column cb + (j & 7)'s), every thread's copy less the bias, and
       // this thread's share of the column sums
-      float m_lane = kNegBig, m_all[16], l_part[16];
+      float m_lane = kNegBig, m_all[kGroupCols], l_part[kGroupCols];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < kGroupCols; ++j) {
         m_all[j] = kNegBig;
         l_part[j] = 0.0f;
       }
       for (int t = t0; t < t1; ++t, ++g) {
         const int buf = g & 1;
-        const int e = g % kScaleStages;
-        if (!mbar_wait(&S.sc_full[e], (g / kScaleStages) & 1, abort, a.err, kErrTimeoutScale)) { ok = false; break; }
-        const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.sc_empty[e]);
-        const float log_vs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
         if (!mbar_wait(&S.s_full[buf], (g >> 1) & 1, abort, a.err, kErrTimeoutS)) { ok = false; break; }
         tc_fence_after();
-        if (t == t0) q_factor = S.q_scale[n & 3] * a.scale_log2;
-        float x[16], x2[16];
-        tmem_ld_32x32b_2x16(tmem + lane_off + buf * 64 + cb, tmem + lane_off + buf * 64 + 32 + cb, x, x2);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.s_free[buf]);
-        const float factor = ks * q_factor;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = fmaf(fmaf(x2[j], 0.0625f, x[j]), factor, log_vs);
         const int key = t * kKeysPerTile + row;
-        if ((t * kKeysPerTile + kKeysPerTile - 1) > min_limit) {
+        if (live) {
+          if (t == t0) q_factor = S.q_scale[n & 3] * a.scale_log2;
+          const int e = g % kScaleStages;
+          const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
+          float x[kGroupCols], x2[kGroupCols];
+          const uint32_t tmem_s = tmem + lane_off + buf * 64 + cb;
+          tmem_ld_32x32b_2x8(tmem_s, tmem_s + kCols, x, x2);
+          const float log_vs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
+          const float factor = ks * q_factor;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int p = (cb + j) / G;
-            const int limit = (a.causal && p < ql) ? L - ql + p : L - 1;
-            x[j] = key <= limit ? x[j] : -INFINITY;
+          for (int j = 0; j < kGroupCols; ++j) x[j] = fmaf(fmaf(x2[j], 0.0625f, x[j]), factor, log_vs);
+          if ((t * kKeysPerTile + kKeysPerTile - 1) > min_limit) {
+#pragma unroll
+            for (int j = 0; j < kGroupCols; ++j) {
+              const int p = (cb + j) / G;
+              const int limit = (a.causal && p < ql) ? L - ql + p : L - 1;
+              x[j] = key <= limit ? x[j] : -INFINITY;
+            }
           }
-        }
-        // ---- does any score of the group pass its column's running maximum by more than 2^8?  Only then (always at an
-        // item's first tile) are the tile's column maxima taken: this warp's, then the four warps'
-        float over = -INFINITY;
+          // ---- does any score of the group pass its column's running maximum by more than 2^8?  Only then (always at an
+          // item's first tile) are the tile's column maxima taken: this warp's, then the four warps'
+          float over = -INFINITY, d[kGroupCols];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) over = fmaxf(over, x[j] - m_all[j]);
-        if (named_barrier_or(bar_wg, 128, over > 8.0f + kPBias)) {
-          float wmax = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float v = warp_max_redux(x[j]);
-            wmax = lane == j ? v : wmax;
+          for (int j = 0; j < kGroupCols; ++j) {
+            d[j] = x[j] - m_all[j];
+            over = fmaxf(over, d[j]);
           }
-          if (lane < 16) S.red_max[buf][col][w] = wmax;
-          named_barrier(bar_wg, 128);
-          const float4 r4 = *reinterpret_cast<const float4*>(S.red_max[buf][col]);
-          const float tmax = fmaxf(fmaxf(r4.x, r4.y), fmaxf(r4.z, r4.w));
-          const float m_new = tmax > m_lane + 8.0f ? tmax : m_lane;
-          const float alpha_lane = ex2_approx(m_lane - m_new);
-          m_lane = m_new;
-          float alpha[16];
+          if (named_barrier_or(bar_wg, 128, over > 8.0f + kPBias)) {
+            float wmax = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            alpha[j] = __shfl_sync(0xffffffffu, alpha_lane, j);
-            m_all[j] = __shfl_sync(0xffffffffu, m_new, j) - kPBias;
-            l_part[j] *= alpha[j];
-          }
-          if (t > t0) {     // O holds this item's earlier tiles: rescale its parts once PV(g-1) has landed
-            if (!mbar_wait(&S.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
-            tc_fence_after();
+            for (int j = 0; j < kGroupCols; ++j) {
+              const float v = warp_max_redux(x[j]);
+              wmax = lane == j ? v : wmax;
+            }
+            if (lane < kGroupCols) S.red_max[buf][col][w] = wmax;
+            named_barrier(bar_wg, 128);
+            const float4 r4 = *reinterpret_cast<const float4*>(S.red_max[buf][col]);
+            const float tmax = fmaxf(fmaxf(r4.x, r4.y), fmaxf(r4.z, r4.w));
+            const float m_new = tmax > m_lane + 8.0f ? tmax : m_lane;
+            const float alpha_lane = ex2_approx(m_lane - m_new);
+            m_lane = m_new;
+            float alpha[kGroupCols];
+#pragma unroll
+            for (int j = 0; j < kGroupCols; ++j) {
+              alpha[j] = __shfl_sync(0xffffffffu, alpha_lane, j);
+              m_all[j] = __shfl_sync(0xffffffffu, m_new, j) - kPBias;
+              l_part[j] *= alpha[j];
+              d[j] = x[j] - m_all[j];
+            }
+            if (t > t0) {     // O holds this item's earlier tiles: rescale its parts once PV(g-1) has landed
+              if (!mbar_wait(&S.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
+              tc_fence_after();
 #pragma unroll 1
-            for (int part = 0; part < kPParts; ++part) {
-              float o[16];
-              tmem_ld_32x32b_x16(tmem_o + part * kCols, o);
+              for (int part = 0; part < kPParts; ++part) {
+                float o[kGroupCols];
+                tmem_ld_32x32b_x8(tmem_o + part * kCols, o);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] *= alpha[j];
-              tmem_st_32x32b_x16(tmem_o + part * kCols, o);
+                for (int j = 0; j < kGroupCols; ++j) o[j] *= alpha[j];
+                tmem_st_32x32b_x8(tmem_o + part * kCols, o);
+              }
             }
           }
-        }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          x[j] = ex2_approx(x[j] - m_all[j]);      // masked: 0
-          l_part[j] = fmaf(x[j], inv_vs, l_part[j]);
-        }
-        // ---- this group's 16 columns of row `row` of the three parts, once PV(g-2) released the buffer
-        if (g >= 2 && !mbar_wait(&S.o_done[buf], ((g - 2) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
-        unsigned char* prow = sP + buf * kPBytes + row * kCols + (wg ^ ((row >> 2) & 1)) * 16;
-#pragma unroll
-        for (int part = 0; part < kPParts; ++part) {
-          unsigned wd[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = x[4 * k + i];
-              y[i] = part < kPParts - 1 ? cut3(v) : v;
-              x[4 * k + i] = v - y[i];
-            }
-            wd[k] = encode_e5m2x2(y[0], y[1]) | encode_e5m2x2(y[2], y[3]) << 16;
+          for (int j = 0; j < kGroupCols; ++j) {
+            x[j] = ex2_approx(d[j]);      // masked: 0
+            l_part[j] = fmaf(x[j], inv_vs, l_part[j]);
           }
-          *reinterpret_cast<uint4*>(prow + part * kPPartBytes) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+          // ---- this group's 8 columns of row `row` of the three parts (S(g) seen: PV(g-2) has released the buffer)
+          unsigned char* prow =
+              sP + buf * kPBytes + row * kCols + ((wg >> 1) ^ ((row >> 2) & 1)) * 16 + (wg & 1) * kGroupCols;
+#pragma unroll
+          for (int part = 0; part < kPParts; ++part) {
+            unsigned wd[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float y[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float v = x[4 * k + i];
+                y[i] = part < kPParts - 1 ? cut3(v) : v;
+                x[4 * k + i] = v - y[i];
+              }
+              wd[k] = encode_e5m2x2(y[0], y[1]) | encode_e5m2x2(y[2], y[3]) << 16;
+            }
+            *reinterpret_cast<uint2*>(prow + part * kPPartBytes) = make_uint2(wd[0], wd[1]);
+          }
         }
-        // ---- the row's last tile: V rows past the context are zeroed; each group zeroes half of the row
+        // ---- the row's last tile: V rows past the context are zeroed; each group zeroes a quarter of the row
         if ((t + 1) * kKeysPerTile > L) {
           const int stage = g % kStages;
           if (!mbar_wait(&S.v_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutV)) { ok = false; break; }
           if (key >= L) {
-            unsigned char* v0 = sV + stage * kTileBytes + row * kHeadDim + wg * 64;
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) *reinterpret_cast<uint4*>(v0 + cc * 16) = make_uint4(0u, 0u, 0u, 0u);
+            unsigned char* v0 = sV + stage * kTileBytes + row * kHeadDim + wg * 32;
+            *reinterpret_cast<uint4*>(v0) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(v0 + 16) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
         fence_proxy_async_smem();
@@ -551,22 +541,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ---- item epilogue: column sums over the 128 key threads, O^T out of TMEM
-      {
-        const float s = column_reduce16(l_part, lane);
-        if (lane < 16) S.red_sum[col][w] = s;
+      if (live) {
+        const float s = column_reduce<kGroupCols>(l_part, lane);
+        if (lane < kGroupCols) S.red_sum[col][w] = s;
       }
       named_barrier(bar_wg, 128);
       const int gl = g - 1;
       if (!mbar_wait(&S.o_done[gl & 1], (gl >> 1) & 1, abort, a.err, kErrTimeoutO)) break;
       tc_fence_after();
-      float o[16];
-      tmem_ld_32x32b_x16(tmem_o, o);
+      float o[kGroupCols];
+      {
+        float o2[kGroupCols], o3[kGroupCols];
+        tmem_ld_32x32b_2x8(tmem_o, tmem_o + kCols, o, o2);
+        tmem_ld_32x32b_x8(tmem_o + 2 * kCols, o3);
 #pragma unroll
-      for (int part = 1; part < kPParts; ++part) {
-        float o2[16];
-        tmem_ld_32x32b_x16(tmem_o + part * kCols, o2);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] += o2[j];
+        for (int j = 0; j < kGroupCols; ++j) o[j] += o2[j] + o3[j];
       }
       tc_fence_before();
       __syncwarp();
@@ -577,33 +566,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long long A = wk.A;
       if (c_lo != c_hi) {
         int* counter = a.counters + (long long)wk.b * a.Hkv + wk.h;
-        if (threadIdx.x == 128) {
+        if (first_thread) {
           const int need = (int)(c_hi - c_lo);
           S.last_piece = (c == c_lo && (seen_early == need || ld_acquire_gpu(counter) == need)) ? 2 : 0;
         }
-        named_barrier(3, 256);
+        named_barrier(kBarMerge, kSoftmaxThreads);
         const bool own_in_registers = S.last_piece == 2;
         if (!own_in_registers) {
           float* mine = a.partial + (2LL * c + (x_begin < A ? 1 : 0)) * kPartialFloats;
+          if (live) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) __stcg(mine + (cb + j) * kHeadDim + row, o[j]);
-          if (w == 0 && lane < 16) {
-            __stcg(mine + kCols * kHeadDim + col, m_lane);
-            __stcg(mine + kCols * kHeadDim + kCols + col, l_lane);
+            for (int j = 0; j < kGroupCols; ++j) __stcg(mine + (cb + j) * kHeadDim + row, o[j]);
+            if (w == 0 && lane < kGroupCols) {
+              __stcg(mine + kCols * kHeadDim + col, m_lane);
+              __stcg(mine + kCols * kHeadDim + kCols + col, l_lane);
+            }
           }
           __threadfence();
-          named_barrier(3, 256);
-          if (threadIdx.x == 128) {
+          named_barrier(kBarMerge, kSoftmaxThreads);             // all groups published
+          if (first_thread) {
             const int last = atomicAdd(counter, 1) == (int)(c_hi - c_lo);
             if (last) atomicExch(counter, 0);
             S.last_piece = last;
           }
-          named_barrier(3, 256);
+          named_barrier(kBarMerge, kSoftmaxThreads);
+          // S.last_piece is next written at the next split item's epilogue, which its writer reaches only after every
+          // softmax warp has handed over P for that item's tiles (so after every thread's read here)
           if (!S.last_piece) continue;
-        } else if (threadIdx.x == 128) {
-          atomicExch(counter, 0);
+        } else if (first_thread) {
+          atomicExch(counter, 0);            // every other piece has arrived: nobody else touches it
         }
         __threadfence();
+        if (!live) continue;
         float m_acc = kNegBig, l_acc = 0.0f;
         const float m_own = m_lane, l_own = l_lane;
         auto merge = [&](float mp, float lp, const float* op) {
@@ -612,17 +606,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_acc = mn;
           l_acc = __fmaf_rn(lp, sb, __fmul_rn(l_acc, sa));
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
+          for (int j = 0; j < kGroupCols; ++j)
             o[j] = __fmaf_rn(op ? __ldcg(op + (cb + j) * kHeadDim + row) : o[j], __shfl_sync(0xffffffffu, sb, j),
                              __fmul_rn(op ? o[j] : 0.0f, __shfl_sync(0xffffffffu, sa, j)));
         };
         long long cc = c_lo;
         if (own_in_registers) {
-          merge(m_own, l_own, nullptr);
+          merge(m_own, l_own, nullptr);      // piece c_lo = this CTA's
           ++cc;
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+          for (int j = 0; j < kGroupCols; ++j) o[j] = 0.0f;
         }
         for (; cc <= c_hi; ++cc) {
           const long long s_cc = T * cc / Ge;
@@ -631,10 +625,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l_lane = l_acc;
       }
+      if (!live) continue;
       const float inv_lane = l_lane > 0.0f ? 1.0f / l_lane : l_lane;      // nothing seen: 0 (and NaN stays)
       const int d = row;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < kGroupCols; ++j) {
         const int p = (cb + j) / G, gq = (cb + j) % G;
         const float inv = __shfl_sync(0xffffffffu, inv_lane, j);
         if (p < ql)

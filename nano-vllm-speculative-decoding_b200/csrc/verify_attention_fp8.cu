@@ -24,9 +24,9 @@
 // The scales never touch the codes: ks_j multiplies the score, and vs_j goes into the exponent: with t_j = s_j + log2 vs_j
 // the running maximum is over t, the tensor core gets p'_j = 2^(t_j - m) (so the largest contribution keeps every bit
 // whatever the scales' spread), and the denominator sums p'_j / vs_j.
-//   warp 0       TMA producer: K tiles and the scales  warps 4-19   softmax over keys (a TMEM lane is a key; four groups of
-//   warp 1       TMEM allocator, MMA issuer                          8 columns each), P parts, O rescale, epilogue
-//   warp 2       prologue                              warps 20-23  query parts of the next items; rows without keys
+//   warp 0       TMA producer: K tiles and the scales  warps 4-11   softmax over keys (a TMEM lane is a key; two groups of
+//   warp 1       TMEM allocator, MMA issuer                          16 columns each), P parts, O rescale, epilogue
+//   warp 2       prologue                              warps 12-15  query parts of the next items; rows without keys
 //   warp 3       TMA producer: the V tiles
 // Softmax: online per column with lazy rescaling (O is rescaled when a column's maximum grows by more than 2^8; p' reaches
 // 2^15 then, in e5m2's range), masked by key index.  V rows past the context are zeroed in shared memory.
@@ -42,12 +42,12 @@ namespace attention_fp8 {
 using namespace attention;
 
 constexpr int kSubKeys = 32;                          // an item's last tile loads in 32-key sub-boxes
-constexpr int kStages = 5;                            // K ring and V ring depth: 160 KB in flight
+constexpr int kStages = 3;                            // K ring and V ring depth: 96 KB in flight
 // Scale ring depth.  A tile's scales arrive on its K tile's barrier.  The entry of tile g is written again for tile
 // g + 8, which K's producer reaches after S(g + 3) is done; S(g + 3) goes out after the softmax has handed over P(g + 1).
 constexpr int kScaleStages = 8;
 static_assert(kScaleStages >= kStages + 2, "a scale entry must outlive the softmax's reads");
-constexpr int kGroups = 4, kGroupCols = kCols / kGroups;   // softmax warpgroups, 8 columns each
+constexpr int kGroups = 2, kGroupCols = kCols / kGroups;   // softmax warpgroups, 16 columns each
 constexpr int kSoftmaxWarp = 4, kSoftmaxThreads = kGroups * 128, kSoftmaxWarps = kSoftmaxThreads / 32;
 constexpr int kQueryWarp = kSoftmaxWarp + kSoftmaxWarps;
 constexpr int kThreads = kQueryWarp * 32 + 128;
@@ -118,11 +118,8 @@ __device__ __forceinline__ float2 decode_e4m3x2(unsigned pair) {
 __device__ __forceinline__ unsigned encode_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ unsigned encode_e5m2x2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E5M2);
-}
-// The value with its mantissa cut to e5m2's two bits (towards zero).
-__device__ __forceinline__ float cut3(float x) { return __uint_as_float(__float_as_uint(x) & 0xffe00000u); }
+__device__ __forceinline__ unsigned half2_bits(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(unsigned u) { return *reinterpret_cast<__half2*>(&u); }
 
 // The page of a row's key, block 0 in place of an id outside the cache.
 __device__ __forceinline__ int page_of(const Args& a, const int* table, int key0) {
@@ -397,11 +394,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= kSoftmaxWarp && ntiles > 0) {
     // ------------------------------------------------------------------ softmax / correction / epilogue
-    const int wg = (warp - kSoftmaxWarp) >> 2;   // column group: columns cb .. cb + 7
+    const int wg = (warp - kSoftmaxWarp) >> 2;   // column group: columns cb .. cb + 15
     const int cb = wg * kGroupCols;
     const int w = warp & 3;                      // TMEM lane quadrant
     const int row = (threadIdx.x - kSoftmaxWarp * 32) & 127;   // key within the tile (S^T) / head dim (O^T)
-    const int col = cb + (lane & 7);             // the column that lane j (and j + 8, ..) speaks for
+    const int col = cb + (lane & 15);            // the column that lane j (and j + 16) speaks for
     const uint32_t lane_off = static_cast<uint32_t>(w * 32) << 16;
     const int bar_wg = 1 + wg;
     const bool first_thread = threadIdx.x == kSoftmaxWarp * 32;
@@ -424,12 +421,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (first_thread && c_lo != c_hi && c == c_lo)
         seen_early = ld_acquire_gpu(a.counters + (long long)wk.b * a.Hkv + wk.h);
       float q_factor = 0.0f;
-      // running maxima of t (log2 domain; lane j owns column cb + (j & 7)'s), every thread's copy less the bias, and
+      // running maxima of t (log2 domain; lane j owns column cb + (j & 15)'s), every thread's copy negated with the bias, and
       // this thread's share of the column sums
-      float m_lane = kNegBig, m_all[kGroupCols], l_part[kGroupCols];
+      float m_lane = kNegBig, m_neg[kGroupCols], l_part[kGroupCols];
 #pragma unroll
       for (int j = 0; j < kGroupCols; ++j) {
-        m_all[j] = kNegBig;
+        m_neg[j] = -kNegBig;
         l_part[j] = 0.0f;
       }
       for (int t = t0; t < t1; ++t, ++g) {
@@ -443,11 +440,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
           float x[kGroupCols], x2[kGroupCols];
           const uint32_t tmem_s = tmem + lane_off + buf * 64 + cb;
-          tmem_ld_32x32b_2x8(tmem_s, tmem_s + kCols, x, x2);
+          tmem_ld_32x32b_2x16(tmem_s, tmem_s + kCols, x, x2);
           const float log_vs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
           const float factor = ks * q_factor;
 #pragma unroll
-          for (int j = 0; j < kGroupCols; ++j) x[j] = fmaf(fmaf(x2[j], 0.0625f, x[j]), factor, log_vs);
+          for (int j = 0; j < kGroupCols; j += 2) {
+            const float2 s = fma_x2(make_float2(x2[j], x2[j + 1]), make_float2(0.0625f, 0.0625f), make_float2(x[j], x[j + 1]));
+            const float2 t2 = fma_x2(s, make_float2(factor, factor), make_float2(log_vs, log_vs));
+            x[j] = t2.x;
+            x[j + 1] = t2.y;
+          }
           if ((t * kKeysPerTile + kKeysPerTile - 1) > min_limit) {
 #pragma unroll
             for (int j = 0; j < kGroupCols; ++j) {
@@ -459,10 +461,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // ---- does any score of the group pass its column's running maximum by more than 2^8?  Only then (always at an
           // item's first tile) are the tile's column maxima taken: this warp's, then the four warps'
           float over = -INFINITY, d[kGroupCols];
+          __half2 ph[kGroupCols / 2];
 #pragma unroll
-          for (int j = 0; j < kGroupCols; ++j) {
-            d[j] = x[j] - m_all[j];
-            over = fmaxf(over, d[j]);
+          for (int j = 0; j < kGroupCols; j += 2) {
+            const float2 d2 = add_x2(make_float2(x[j], x[j + 1]), make_float2(m_neg[j], m_neg[j + 1]));
+            d[j] = d2.x;
+            d[j + 1] = d2.y;
+            over = fmaxf(fmaxf(over, d2.x), d2.y);
           }
           if (named_barrier_or(bar_wg, 128, over > 8.0f + kPBias)) {
             float wmax = -INFINITY;
@@ -482,9 +487,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < kGroupCols; ++j) {
               alpha[j] = __shfl_sync(0xffffffffu, alpha_lane, j);
-              m_all[j] = __shfl_sync(0xffffffffu, m_new, j) - kPBias;
+              m_neg[j] = kPBias - __shfl_sync(0xffffffffu, m_new, j);
               l_part[j] *= alpha[j];
-              d[j] = x[j] - m_all[j];
+              d[j] = x[j] + m_neg[j];
             }
             if (t > t0) {     // O holds this item's earlier tiles: rescale its parts once PV(g-1) has landed
               if (!mbar_wait(&S.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
@@ -492,46 +497,51 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
               for (int part = 0; part < kPParts; ++part) {
                 float o[kGroupCols];
-                tmem_ld_32x32b_x8(tmem_o + part * kCols, o);
+                tmem_ld_32x32b_x16(tmem_o + part * kCols, o);
 #pragma unroll
                 for (int j = 0; j < kGroupCols; ++j) o[j] *= alpha[j];
-                tmem_st_32x32b_x8(tmem_o + part * kCols, o);
+                tmem_st_32x32b_x16(tmem_o + part * kCols, o);
               }
             }
           }
 #pragma unroll
-          for (int j = 0; j < kGroupCols; ++j) {
-            x[j] = ex2_approx(d[j]);      // masked: 0
-            l_part[j] = fmaf(x[j], inv_vs, l_part[j]);
+          for (int j = 0; j < kGroupCols; j += 2) {
+            const float2 p2 = make_float2(ex2_approx(d[j]), ex2_approx(d[j + 1]));      // masked: 0
+            const float2 l2 = fma_x2(p2, make_float2(inv_vs, inv_vs), make_float2(l_part[j], l_part[j + 1]));
+            l_part[j] = l2.x;
+            l_part[j + 1] = l2.y;
+            ph[j / 2] = __floats2half2_rn(p2.x, p2.y);
           }
-          // ---- this group's 8 columns of row `row` of the three parts (S(g) seen: PV(g-2) has released the buffer)
-          unsigned char* prow =
-              sP + buf * kPBytes + row * kCols + ((wg >> 1) ^ ((row >> 2) & 1)) * 16 + (wg & 1) * kGroupCols;
+          // ---- this group's 16 columns of row `row` of the three parts (S(g) seen: PV(g-2) has released the buffer)
+          // An fp16 pattern's high byte is its value cut to e5m2; what is left over is exact in fp16.  Two cuts, then the
+          // third part to nearest: p is fp16's 2^-12 and e5m2's last half step, 2^-9 of p, from p'.
+          unsigned char* prow = sP + buf * kPBytes + row * kCols + (wg ^ ((row >> 2) & 1)) * 16;
 #pragma unroll
           for (int part = 0; part < kPParts; ++part) {
-            unsigned wd[2];
+            unsigned wd[4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float y[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float v = x[4 * k + i];
-                y[i] = part < kPParts - 1 ? cut3(v) : v;
-                x[4 * k + i] = v - y[i];
+            for (int k = 0; k < 4; ++k) {
+              unsigned lo = half2_bits(ph[2 * k]), hi = half2_bits(ph[2 * k + 1]);
+              if (part == kPParts - 1) {
+                lo += 0x00800080u;
+                hi += 0x00800080u;
+              } else {
+                ph[2 * k] = __hsub2(ph[2 * k], bits_half2(lo & 0xff00ff00u));
+                ph[2 * k + 1] = __hsub2(ph[2 * k + 1], bits_half2(hi & 0xff00ff00u));
               }
-              wd[k] = encode_e5m2x2(y[0], y[1]) | encode_e5m2x2(y[2], y[3]) << 16;
+              wd[k] = __byte_perm(lo, hi, 0x7531);
             }
-            *reinterpret_cast<uint2*>(prow + part * kPPartBytes) = make_uint2(wd[0], wd[1]);
+            *reinterpret_cast<uint4*>(prow + part * kPPartBytes) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
           }
         }
-        // ---- the row's last tile: V rows past the context are zeroed; each group zeroes a quarter of the row
+        // ---- the row's last tile: V rows past the context are zeroed; each group zeroes half of the row
         if ((t + 1) * kKeysPerTile > L) {
           const int stage = g % kStages;
           if (!mbar_wait(&S.v_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutV)) { ok = false; break; }
           if (key >= L) {
-            unsigned char* v0 = sV + stage * kTileBytes + row * kHeadDim + wg * 32;
-            *reinterpret_cast<uint4*>(v0) = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(v0 + 16) = make_uint4(0u, 0u, 0u, 0u);
+            unsigned char* v0 = sV + stage * kTileBytes + row * kHeadDim + wg * 64;
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) *reinterpret_cast<uint4*>(v0 + cc * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
         fence_proxy_async_smem();
@@ -552,8 +562,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float o[kGroupCols];
       {
         float o2[kGroupCols], o3[kGroupCols];
-        tmem_ld_32x32b_2x8(tmem_o, tmem_o + kCols, o, o2);
-        tmem_ld_32x32b_x8(tmem_o + 2 * kCols, o3);
+        tmem_ld_32x32b_2x16(tmem_o, tmem_o + kCols, o, o2);
+        tmem_ld_32x32b_x16(tmem_o + 2 * kCols, o3);
 #pragma unroll
         for (int j = 0; j < kGroupCols; ++j) o[j] += o2[j] + o3[j];
       }

@@ -175,15 +175,31 @@ __device__ __forceinline__ void mma_bf16_ss(uint32_t d_tmem, uint64_t a_desc, ui
 }
 // D[tmem] (+)= A[smem] * B[smem], kind::f8f6f4 (8-bit floats, each operand e4m3 or e5m2, fp32 accumulate), one CTA.
 // The descriptors come as their two words: an issuing loop keeps the high ones and steps the low ones (addresses).
-__device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
-                                          uint32_t idesc, uint32_t accumulate) {
+// Called by a whole warp, whose one elected lane (leader) issues: the operands then stay in uniform registers, and the
+// instruction is predicated, not branched around.
+__device__ __forceinline__ void mma_f8_ss(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                          uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
+      "{\n\t.reg .pred p, l;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 l, %7, 0;\n\t"
       "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      "@l tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
+}
+// mma_commit by a whole warp's elected lane.
+__device__ __forceinline__ void mma_commit_leader(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %1, 0;\n\t"
+      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+// 1 in one lane of a converged warp, the same one at every call; 0 in the others.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 // Arrives on the mbarrier once every tcgen05 operation this thread issued before has completed.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {

@@ -254,33 +254,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && ntiles > 0) {
+    // ------------------------------------------------------------------ MMA issuer: the whole warp, one lane issuing
+    if (ntiles > 0) {
       constexpr uint32_t idesc_s = idesc_f8_f32(128, kQParts * kCols, 0, 0, 0, 0);    // e4m3 . e4m3
       constexpr uint32_t idesc_o = idesc_f8_f32(128, kPParts * kCols, 0, 1, 1, 1);    // e4m3 . e5m2
+      constexpr unsigned kAll = 0xffffffffu;
+      const uint32_t leader = elect_one();
       // descriptors of the first buffers; the others differ in the low word's address (16-byte units)
       const uint64_t kd = smem_desc(sK, 16, 1024, kSwizzle128B), qd = smem_desc(sQ, 16, 1024, kSwizzle128B);
       const uint64_t vd = smem_desc(sV, kTileBytes, 1024, kSwizzle128B), pd = smem_desc(sP, kPPartBytes, 256, kSwizzle32B);
       const uint32_t kd_hi = (uint32_t)(kd >> 32), qd_hi = (uint32_t)(qd >> 32), vd_hi = (uint32_t)(vd >> 32),
                      pd_hi = (uint32_t)(pd >> 32);
+      const uint32_t tm = __shfl_sync(kAll, tmem, 0);
+      const int count = __shfl_sync(kAll, ntiles, 0);
       Cursor<QMAX, true> cs, cp;     // the score MMAs run two tiles ahead of the PV MMAs
       cs.start(a, S);
       cp.start(a, S);
       int sk = 0, sv = 0;            // ring stages of the next K and V tile, and their phases
       uint32_t sk_phase = 0, sv_phase = 0;
+      int qn = 0, on = 0;            // the cursors' segment numbers, warp-uniform
+      auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
+        return __all_sync(kAll, mbar_wait(bar, phase, abort, a.err, code));
+      };
       auto issue_s = [&](int g) -> bool {
-        const int qb = cs.n & 1;
-        if (cs.first && !mbar_wait(&S.q_full[qb], (cs.n >> 1) & 1, abort, a.err, kErrTimeoutQ)) return false;
-        if (!mbar_wait(&S.k_full[sk], sk_phase, abort, a.err, kErrTimeoutK)) return false;
+        const int qb = qn & 1;
+        if (__any_sync(kAll, cs.first) && !wait(&S.q_full[qb], (qn >> 1) & 1, kErrTimeoutQ)) return false;
+        if (!wait(&S.k_full[sk], sk_phase, kErrTimeoutK)) return false;
         tc_fence_after();
         const uint32_t ka = (uint32_t)kd + sk * (kTileBytes >> 4), qa = (uint32_t)qd + qb * (kQBytes >> 4);
-        const uint32_t tmem_s = tmem + (g & 1) * 64;
+        const uint32_t tmem_s = tm + (g & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < kHeadDim / 32; ++kk)
-          mma_f8_ss(tmem_s, ka + kk * 2, kd_hi, qa + kk * 2, qd_hi, idesc_s, kk > 0 ? 1u : 0u);
-        mma_commit(&S.s_full[g & 1]);
-        mma_commit(&S.k_empty[sk]);
-        if (cs.last()) mma_commit(&S.q_empty[qb]);
+          mma_f8_ss(leader, tmem_s, ka + kk * 2, kd_hi, qa + kk * 2, qd_hi, idesc_s, kk > 0 ? 1u : 0u);
+        mma_commit_leader(leader, &S.s_full[g & 1]);
+        mma_commit_leader(leader, &S.k_empty[sk]);
+        if (__any_sync(kAll, cs.last())) {
+          mma_commit_leader(leader, &S.q_empty[qb]);
+          ++qn;
+        }
         if (++sk == kStages) {
           sk = 0;
           sk_phase ^= 1;
@@ -289,35 +300,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       auto issue_pv = [&](int g) -> bool {
-        const int ob = cp.n & 1;
-        if (cp.first && cp.n >= 2 && !mbar_wait(&S.o_free[ob], ((cp.n - 2) >> 1) & 1, abort, a.err, kErrTimeoutO))
-          return false;
-        if (!mbar_wait(&S.v_full[sv], sv_phase, abort, a.err, kErrTimeoutV)) return false;
-        if (!mbar_wait(&S.p_full[g & 1], (g >> 1) & 1, abort, a.err, kErrTimeoutP)) return false;
+        const int ob = on & 1;
+        const bool fresh = __any_sync(kAll, cp.first);
+        if (fresh && on >= 2 && !wait(&S.o_free[ob], ((on - 2) >> 1) & 1, kErrTimeoutO)) return false;
+        if (!wait(&S.v_full[sv], sv_phase, kErrTimeoutV)) return false;
+        if (!wait(&S.p_full[g & 1], (g >> 1) & 1, kErrTimeoutP)) return false;
         tc_fence_after();
         const uint32_t va = (uint32_t)vd + sv * (kTileBytes >> 4), pa = (uint32_t)pd + (g & 1) * (kPBytes >> 4);
-        const uint32_t tmem_o = tmem + kTmemO + ob * kTmemOStride;
-        const uint32_t fresh = cp.first ? 0u : 1u;
+        const uint32_t tmem_o = tm + kTmemO + ob * kTmemOStride;
 #pragma unroll
         for (int kk = 0; kk < kKeysPerTile / 32; ++kk)
-          mma_f8_ss(tmem_o, va + kk * (32 * kHeadDim >> 4), vd_hi, pa + kk * (32 * kCols >> 4), pd_hi, idesc_o,
-                    kk > 0 ? 1u : fresh);
-        mma_commit(&S.o_done[g & 1]);
-        mma_commit(&S.v_empty[sv]);
+          mma_f8_ss(leader, tmem_o, va + kk * (32 * kHeadDim >> 4), vd_hi, pa + kk * (32 * kCols >> 4), pd_hi, idesc_o,
+                    kk > 0 || !fresh ? 1u : 0u);
+        mma_commit_leader(leader, &S.o_done[g & 1]);
+        mma_commit_leader(leader, &S.v_empty[sv]);
         if (++sv == kStages) {
           sv = 0;
           sv_phase ^= 1;
         }
+        if (__any_sync(kAll, cp.last())) ++on;
         cp.advance(a, x_begin, x_end);
         return true;
       };
       // PV(g) goes out before S(g + 2).  The wait for P(g) says that the softmax has read S(g) and the tile's scales, so
       // S's buffer is free; and as MMAs complete in order, a softmax that sees S(g + 2) knows that PV(g) has read P's.
       bool ok = issue_s(0);
-      if (ok && ntiles > 1) ok = issue_s(1);
-      for (int g = 0; g < ntiles && ok; ++g) {
+      if (ok && count > 1) ok = issue_s(1);
+      for (int g = 0; g < count && ok; ++g) {
         ok = issue_pv(g);
-        if (ok && g + 2 < ntiles) ok = issue_s(g + 2);
+        if (ok && g + 2 < count) ok = issue_s(g + 2);
       }
     }
   } else if (warp >= kQueryWarp) {
@@ -608,30 +619,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __threadfence();
         if (!live) continue;
-        float m_acc = kNegBig, l_acc = 0.0f;
-        const float m_own = m_lane, l_own = l_lane;
-        auto merge = [&](float mp, float lp, const float* op) {
-          const float mn = fmaxf(m_acc, mp);
-          const float sa = ex2_approx(m_acc - mn), sb = ex2_approx(mp - mn);
-          m_acc = mn;
-          l_acc = __fmaf_rn(lp, sb, __fmul_rn(l_acc, sa));
-#pragma unroll
-          for (int j = 0; j < kGroupCols; ++j)
-            o[j] = __fmaf_rn(op ? __ldcg(op + (cb + j) * kHeadDim + row) : o[j], __shfl_sync(0xffffffffu, sb, j),
-                             __fmul_rn(op ? o[j] : 0.0f, __shfl_sync(0xffffffffu, sa, j)));
+        // pieces in CTA order, the common maximum first so that the pieces' loads do not wait for one another
+        auto piece_of = [&](long long cc) {
+          return a.partial + (2 * cc + (T * cc / Ge < A ? 1 : 0)) * kPartialFloats;
         };
-        long long cc = c_lo;
-        if (own_in_registers) {
-          merge(m_own, l_own, nullptr);      // piece c_lo = this CTA's
-          ++cc;
+        const float m_own = m_lane, l_own = l_lane;
+        float m_acc = own_in_registers ? m_own : kNegBig;
+        const long long c_from = c_lo + (own_in_registers ? 1 : 0);
+#pragma unroll 4
+        for (long long cc = c_from; cc <= c_hi; ++cc) m_acc = fmaxf(m_acc, __ldcg(piece_of(cc) + kCols * kHeadDim + col));
+        float l_acc = 0.0f;
+        if (own_in_registers) {              // piece c_lo = this CTA's
+          const float sb = ex2_approx(m_own - m_acc);
+          l_acc = __fmul_rn(l_own, sb);
+#pragma unroll
+          for (int j = 0; j < kGroupCols; ++j) o[j] = __fmul_rn(o[j], __shfl_sync(0xffffffffu, sb, j));
         } else {
 #pragma unroll
           for (int j = 0; j < kGroupCols; ++j) o[j] = 0.0f;
         }
-        for (; cc <= c_hi; ++cc) {
-          const long long s_cc = T * cc / Ge;
-          const float* piece = a.partial + (2 * cc + (s_cc < A ? 1 : 0)) * kPartialFloats;
-          merge(__ldcg(piece + kCols * kHeadDim + col), __ldcg(piece + kCols * kHeadDim + kCols + col), piece);
+#pragma unroll 2
+        for (long long cc = c_from; cc <= c_hi; ++cc) {
+          const float* piece = piece_of(cc);
+          const float mp = __ldcg(piece + kCols * kHeadDim + col), lp = __ldcg(piece + kCols * kHeadDim + kCols + col);
+          float op[kGroupCols];
+#pragma unroll
+          for (int j = 0; j < kGroupCols; ++j) op[j] = __ldcg(piece + (cb + j) * kHeadDim + row);
+          const float sb = ex2_approx(mp - m_acc);
+          l_acc = __fmaf_rn(lp, sb, l_acc);
+#pragma unroll
+          for (int j = 0; j < kGroupCols; ++j) o[j] = __fmaf_rn(op[j], __shfl_sync(0xffffffffu, sb, j), o[j]);
         }
         l_lane = l_acc;
       }

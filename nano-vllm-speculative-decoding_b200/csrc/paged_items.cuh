@@ -139,7 +139,7 @@ struct Walk {
   __device__ __forceinline__ void start(const Args& a, const Smem& S) {
     b = S.b_start;
     r = RowInfo{S.r0[0], S.r0[1], S.r0[2], S.r0[3]};   // found by the prologue
-    h = (int)((S.x_begin - S.row_tile0) / r.nt);
+    h = (int)(S.x_begin - S.row_tile0) / r.nt;        // within the row: nt * Hkv tiles, 32 bits
     A = S.row_tile0 + (long long)h * r.nt;
   }
   template <typename Args>
@@ -188,6 +188,14 @@ struct Cursor {
   }
 };
 
+// x * y / z for y and z up to the grid (< 256): in 32 bits where the product fits, as it does below 2^24 tiles.
+__device__ __forceinline__ long long mul_div(long long x, long long y, long long z) {
+  return x < (1LL << 24) ? (long long)((unsigned)x * (unsigned)y / (unsigned)z) : x * y / z;
+}
+// ceil(x * y / z) for y up to the grid (< 256) and x up to z: the same.
+__device__ __forceinline__ long long mul_ceil_div(long long x, long long y, long long z) {
+  return z < (1LL << 24) ? (long long)(((unsigned)x * (unsigned)y + (unsigned)z - 1u) / (unsigned)z) : (x * y + z - 1) / z;
+}
 __device__ __forceinline__ long long ceil_div(long long x, long long y) { return (x + y - 1) / y; }
 
 // This CTA's share [xb, xe) of the tile sequence, split evenly over Ge = min(grid, T) CTAs, and the row holding its
@@ -212,8 +220,8 @@ __device__ __forceinline__ Share find_share(const Args& a, int lane) {
   int bstart = 0;
   RowInfo r0{0, 0, 0, 1};
   if (c < Ge) {
-    xb = T * c / Ge;
-    xe = T * (c + 1) / Ge;
+    xb = mul_div(T, c, Ge);
+    xe = mul_div(T, c + 1, Ge);
     long long pre = 0;
     for (int b0 = 0; b0 < a.R; b0 += 32) {
       const int b = b0 + lane;

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int page0 = 0;
       if (share.xe > share.xb) {       // the share's first tile: its page, and its codes into L2 ahead of the loads
-        const int h = (int)((share.xb - share.row0) / share.r0.nt);
+        const int h = (int)(share.xb - share.row0) / share.r0.nt;
         const int key0 = (int)(share.xb - share.row0 - (long long)h * share.r0.nt) * kKeysPerTile;
         page0 = page_of(a, a.block_tables + (long long)share.bstart * a.W, key0);
         tma_prefetch_3d(&kmap, 0, key0 % a.block_size, page0 * a.Hkv + h);
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int min_limit = a.causal ? L - ql : L - 1;       // smallest limit among the valid columns
       // A group none of whose columns holds a query only keeps the barriers going: its columns of P and O are never read.
       const bool live = cb < ql * G;
-      const long long c_lo = ceil_div((wk.A + 1) * Ge, T) - 1, c_hi = ceil_div((wk.A + wk.r.nt) * Ge, T) - 1;
+      const long long c_lo = mul_ceil_div(wk.A + 1, Ge, T) - 1, c_hi = mul_ceil_div(wk.A + wk.r.nt, Ge, T) - 1;
       int seen_early = -1;
       if (first_thread && c_lo != c_hi && c == c_lo)
         seen_early = ld_acquire_gpu(a.counters + (long long)wk.b * a.Hkv + wk.h);
@@ -620,8 +620,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __threadfence();
         if (!live) continue;
         // pieces in CTA order, the common maximum first so that the pieces' loads do not wait for one another
+        // (only the first piece's CTA can hold an earlier item before it)
+        const int c_lo_slot = mul_div(T, c_lo, Ge) < A ? 1 : 0;
         auto piece_of = [&](long long cc) {
-          return a.partial + (2 * cc + (T * cc / Ge < A ? 1 : 0)) * kPartialFloats;
+          return a.partial + (2 * cc + (cc == c_lo ? c_lo_slot : 0)) * kPartialFloats;
         };
         const float m_own = m_lane, l_own = l_lane;
         float m_acc = own_in_registers ? m_own : kNegBig;

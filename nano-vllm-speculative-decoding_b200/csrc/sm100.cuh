@@ -125,6 +125,16 @@ __device__ __forceinline__ void fence_proxy_async_global() {
   asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
+// Gives up / takes registers, by a whole warpgroup: a block's shares must stay within its threads x registers at launch.
+template <int kRegs>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 // Named barrier over `count` threads (count a multiple of 32).
 __device__ __forceinline__ void named_barrier(int id, int count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
@@ -266,21 +276,34 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const float (
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// Two such blocks of 16 columns, one wait for both.
-__device__ __forceinline__ void tmem_ld_32x32b_2x16(uint32_t ta, uint32_t tb, float (&a)[16], float (&b)[16]) {
-  uint32_t r[16], s[16];
+// Two such blocks of 16 columns; the registers hold them only after tmem_ld_wait_2x16.
+__device__ __forceinline__ void tmem_ld_start_2x16(uint32_t ta, uint32_t tb, uint32_t (&r)[16], uint32_t (&s)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
       "%15}, [%32];\n\t"
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%33];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "%30, %31}, [%33];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(s[0]), "=r"(s[1]), "=r"(s[2]), "=r"(s[3]), "=r"(s[4]), "=r"(s[5]), "=r"(s[6]), "=r"(s[7]),
         "=r"(s[8]), "=r"(s[9]), "=r"(s[10]), "=r"(s[11]), "=r"(s[12]), "=r"(s[13]), "=r"(s[14]), "=r"(s[15])
       : "r"(ta), "r"(tb)
       : "memory");
+}
+// The registers pass through the wait, so that no use of them can move before it.
+__device__ __forceinline__ void tmem_ld_wait_2x16(uint32_t (&r)[16], uint32_t (&s)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(s[0]), "+r"(s[1]), "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7]),
+                 "+r"(s[8]), "+r"(s[9]), "+r"(s[10]), "+r"(s[11]), "+r"(s[12]), "+r"(s[13]), "+r"(s[14]), "+r"(s[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_2x16(uint32_t ta, uint32_t tb, float (&a)[16], float (&b)[16]) {
+  uint32_t r[16], s[16];
+  tmem_ld_start_2x16(ta, tb, r, s);
+  tmem_ld_wait_2x16(r, s);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     a[i] = __uint_as_float(r[i]);

@@ -30,6 +30,11 @@
 //   warp 3       TMA producer: the V tiles
 // Softmax: online per column with lazy rescaling (O is rescaled when a column's maximum grows by more than 2^8; p' reaches
 // 2^15 then, in e5m2's range), masked by key index.  V rows past the context are zeroed in shared memory.
+// A softmax step takes a pair of tiles: its fixed costs (score load, the vote on the maxima, the proxy fence, the
+// hand-over: some 700 clocks that two warps a scheduler cannot hide) are paid once for 256 keys, and a warp has two
+// independent tiles' arithmetic to interleave (16k contexts: 379 -> 362 us; one tile ahead in software instead: 595 us).
+// The MMA warp runs converged with a predicated leader lane: issued from a divergent lane an MMA cost about 100 clocks,
+// more than its execution (429 -> 376 us).  Rings deeper than this lost time (5 stages of K and V: 15 % at 3k contexts).
 #include "paged_items.cuh"
 #include "specdec_b200.h"
 
@@ -42,23 +47,28 @@ namespace attention_fp8 {
 using namespace attention;
 
 constexpr int kSubKeys = 32;                          // an item's last tile loads in 32-key sub-boxes
-constexpr int kStages = 3;                            // K ring and V ring depth: 96 KB in flight
+constexpr int kStages = 4;                            // K ring and V ring depth (tiles): 128 KB in flight
 // Scale ring depth.  A tile's scales arrive on its K tile's barrier.  The entry of tile g is written again for tile
-// g + 8, which K's producer reaches after S(g + 3) is done; S(g + 3) goes out after the softmax has handed over P(g + 1).
-constexpr int kScaleStages = 8;
-static_assert(kScaleStages >= kStages + 2, "a scale entry must outlive the softmax's reads");
+// g + 16, which K's producer reaches after S of tile g + 12 is done: at least six pairs on, and a pair's scores go out
+// after P of the pair two before it.
+constexpr int kScaleStages = 16;
+static_assert(kScaleStages >= kStages + 4, "a scale entry must outlive the softmax's reads");
 constexpr int kGroups = 2, kGroupCols = kCols / kGroups;   // softmax warpgroups, 16 columns each
 constexpr int kSoftmaxWarp = 4, kSoftmaxThreads = kGroups * 128, kSoftmaxWarps = kSoftmaxThreads / 32;
 constexpr int kQueryWarp = kSoftmaxWarp + kSoftmaxWarps;
 constexpr int kThreads = kQueryWarp * 32 + 128;
+// The softmax holds a pair of tiles in registers: the other warpgroups (0: producers and MMA, 3: queries) hand theirs over.
+// The shares must fit what the block is launched with, which the host checks.
+constexpr int kSoftmaxRegs = 168, kProducerRegs = 72;
+constexpr int kLaunchRegs = (kSoftmaxRegs * kSoftmaxThreads + kProducerRegs * 256 + kThreads - 1) / kThreads;
 constexpr int kBarMerge = 1 + kGroups, kBarQuery = 2 + kGroups;   // named barriers: 1 .. kGroups are the groups'
 constexpr int kTileBytes = kKeysPerTile * kHeadDim;   // 16 KB of codes
 constexpr int kQParts = 2, kPParts = 3;
 constexpr int kQBytes = kQParts * kCols * kHeadDim;   // 8 KB, double-buffered by item
 constexpr int kPPartBytes = kKeysPerTile * kCols;     // 4 KB
-constexpr int kPBytes = kPParts * kPPartBytes;        // 12 KB, double-buffered by tile
-constexpr uint32_t kTmemCols = 512;                   // S0 at 0, S1 at 64; O0 at 128, O1 at 256 (96 columns each)
-constexpr uint32_t kTmemO = 128, kTmemOStride = 128;
+constexpr int kPBytes = kPParts * kPPartBytes;        // 12 KB a tile; a pair's 24 KB double-buffered
+constexpr uint32_t kTmemCols = 512;                   // two pairs of S (2 x 64 columns), then O0 and O1 of 96
+constexpr uint32_t kTmemSTile = 64, kTmemSPair = 128, kTmemO = 256, kTmemOStride = 128;
 constexpr float kPBias = 7.0f;                        // p' is kept 2^7 up: its range is [2^-24, 2^8] of the maximum
 constexpr float kMinScale = 7.888609052210118e-31f;   // 2^-100, the store's smallest scale
 
@@ -91,7 +101,7 @@ struct Smem {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
   alignas(16) float scales[kScaleStages][2][kKeysPerTile / 16];   // [ring][K, V][group of the tile]
-  alignas(16) float red_max[2][32][4];   // [tile parity][column][warp] maxima
+  alignas(16) float red_max[2][32][4];   // [pair parity][column][warp] maxima
   alignas(16) float red_sum[32][4];
   unsigned red_q[4];
   float q_scale[4];          // by item & 3: the item's 2^e
@@ -108,7 +118,7 @@ constexpr int kOffQ = 0;
 constexpr int kOffK = kOffQ + 2 * kQBytes;
 constexpr int kOffV = kOffK + kStages * kTileBytes;
 constexpr int kOffP = kOffV + kStages * kTileBytes;
-constexpr int kOffCtl = kOffP + 2 * kPBytes;
+constexpr int kOffCtl = kOffP + 4 * kPBytes;
 constexpr int kSmemBytes = kOffCtl + (int)sizeof(Smem) + 1024;   // + alignment slack
 static_assert(kSmemBytes <= 232448, "shared memory above the sm_100 per-CTA limit");
 
@@ -130,6 +140,32 @@ __device__ __forceinline__ int page_of(const Args& a, const int* table, int key0
   }
   return page;
 }
+
+// Pair-by-pair cursor over the CTA's share: the segment (item piece) number n, whether the pair is its first or last, and
+// whether it has a second tile (a piece of an odd number of tiles ends in a single).
+template <int QMAX>
+struct PairCursor {
+  Walk<QMAX, true> w;
+  int n, left;
+  bool first;
+  __device__ __forceinline__ void start(const Args& a, const Smem& S) {
+    w.start(a, S);
+    n = 0;
+    left = w.t1(S.x_end) - w.t0(S.x_begin);
+    first = true;
+  }
+  __device__ __forceinline__ bool two() const { return left >= 2; }
+  __device__ __forceinline__ bool last() const { return left <= 2; }
+  __device__ __forceinline__ void advance(const Args& a, long long x_begin, long long x_end) {
+    first = last();
+    left -= 2;
+    if (left <= 0) {
+      w.next(a);
+      ++n;
+      left = w.t1(x_end) - w.t0(x_begin);
+    }
+  }
+};
 
 template <int G>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -207,7 +243,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort = &S.abort;
   const long long x_begin = S.x_begin, x_end = S.x_end;
   const int ntiles = (int)(x_end - x_begin);
+  const bool softmax = warp >= kSoftmaxWarp && warp < kQueryWarp;
 
+  if (!softmax) registers_down<kProducerRegs>();
   if (warp == 0 || warp == 3) {
     // ------------------------------------------------------------------ TMA producers: K with both scales, V
     const bool is_k = warp == 0;
@@ -267,68 +305,78 @@ __global__ void __launch_bounds__(kThreads, 1)
                      pd_hi = (uint32_t)(pd >> 32);
       const uint32_t tm = __shfl_sync(kAll, tmem, 0);
       const int count = __shfl_sync(kAll, ntiles, 0);
-      Cursor<QMAX, true> cs, cp;     // the score MMAs run two tiles ahead of the PV MMAs
+      PairCursor<QMAX> cs, cp;       // the score MMAs run two pairs ahead of the PV MMAs
       cs.start(a, S);
       cp.start(a, S);
       int sk = 0, sv = 0;            // ring stages of the next K and V tile, and their phases
       uint32_t sk_phase = 0, sv_phase = 0;
       int qn = 0, on = 0;            // the cursors' segment numbers, warp-uniform
+      int done_s = 0, done_pv = 0;   // tiles issued
       auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
         return __all_sync(kAll, mbar_wait(bar, phase, abort, a.err, code));
       };
-      auto issue_s = [&](int g) -> bool {
+      auto issue_s = [&](int u) -> bool {        // scores of pair u
         const int qb = qn & 1;
+        const bool two = __any_sync(kAll, cs.two());
         if (__any_sync(kAll, cs.first) && !wait(&S.q_full[qb], (qn >> 1) & 1, kErrTimeoutQ)) return false;
-        if (!wait(&S.k_full[sk], sk_phase, kErrTimeoutK)) return false;
-        tc_fence_after();
-        const uint32_t ka = (uint32_t)kd + sk * (kTileBytes >> 4), qa = (uint32_t)qd + qb * (kQBytes >> 4);
-        const uint32_t tmem_s = tm + (g & 1) * 64;
+        const uint32_t qa = (uint32_t)qd + qb * (kQBytes >> 4);
+        for (int i = 0; i < (two ? 2 : 1); ++i) {
+          if (!wait(&S.k_full[sk], sk_phase, kErrTimeoutK)) return false;
+          tc_fence_after();
+          const uint32_t ka = (uint32_t)kd + sk * (kTileBytes >> 4);
+          const uint32_t tmem_s = tm + (u & 1) * kTmemSPair + i * kTmemSTile;
 #pragma unroll
-        for (int kk = 0; kk < kHeadDim / 32; ++kk)
-          mma_f8_ss(leader, tmem_s, ka + kk * 2, kd_hi, qa + kk * 2, qd_hi, idesc_s, kk > 0 ? 1u : 0u);
-        mma_commit_leader(leader, &S.s_full[g & 1]);
-        mma_commit_leader(leader, &S.k_empty[sk]);
+          for (int kk = 0; kk < kHeadDim / 32; ++kk)
+            mma_f8_ss(leader, tmem_s, ka + kk * 2, kd_hi, qa + kk * 2, qd_hi, idesc_s, kk > 0 ? 1u : 0u);
+          mma_commit_leader(leader, &S.k_empty[sk]);
+          if (++sk == kStages) {
+            sk = 0;
+            sk_phase ^= 1;
+          }
+        }
+        mma_commit_leader(leader, &S.s_full[u & 1]);
         if (__any_sync(kAll, cs.last())) {
           mma_commit_leader(leader, &S.q_empty[qb]);
           ++qn;
         }
-        if (++sk == kStages) {
-          sk = 0;
-          sk_phase ^= 1;
-        }
+        done_s += two ? 2 : 1;
         cs.advance(a, x_begin, x_end);
         return true;
       };
-      auto issue_pv = [&](int g) -> bool {
+      auto issue_pv = [&](int u) -> bool {
         const int ob = on & 1;
-        const bool fresh = __any_sync(kAll, cp.first);
+        const bool two = __any_sync(kAll, cp.two()), fresh = __any_sync(kAll, cp.first);
         if (fresh && on >= 2 && !wait(&S.o_free[ob], ((on - 2) >> 1) & 1, kErrTimeoutO)) return false;
-        if (!wait(&S.v_full[sv], sv_phase, kErrTimeoutV)) return false;
-        if (!wait(&S.p_full[g & 1], (g >> 1) & 1, kErrTimeoutP)) return false;
-        tc_fence_after();
-        const uint32_t va = (uint32_t)vd + sv * (kTileBytes >> 4), pa = (uint32_t)pd + (g & 1) * (kPBytes >> 4);
+        if (!wait(&S.p_full[u & 1], (u >> 1) & 1, kErrTimeoutP)) return false;
         const uint32_t tmem_o = tm + kTmemO + ob * kTmemOStride;
+        for (int i = 0; i < (two ? 2 : 1); ++i) {
+          if (!wait(&S.v_full[sv], sv_phase, kErrTimeoutV)) return false;
+          tc_fence_after();
+          const uint32_t va = (uint32_t)vd + sv * (kTileBytes >> 4), pa = (uint32_t)pd + ((u & 1) * 2 + i) * (kPBytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kKeysPerTile / 32; ++kk)
-          mma_f8_ss(leader, tmem_o, va + kk * (32 * kHeadDim >> 4), vd_hi, pa + kk * (32 * kCols >> 4), pd_hi, idesc_o,
-                    kk > 0 || !fresh ? 1u : 0u);
-        mma_commit_leader(leader, &S.o_done[g & 1]);
-        mma_commit_leader(leader, &S.v_empty[sv]);
-        if (++sv == kStages) {
-          sv = 0;
-          sv_phase ^= 1;
+          for (int kk = 0; kk < kKeysPerTile / 32; ++kk)
+            mma_f8_ss(leader, tmem_o, va + kk * (32 * kHeadDim >> 4), vd_hi, pa + kk * (32 * kCols >> 4), pd_hi, idesc_o,
+                      kk > 0 || i > 0 || !fresh ? 1u : 0u);
+          mma_commit_leader(leader, &S.v_empty[sv]);
+          if (++sv == kStages) {
+            sv = 0;
+            sv_phase ^= 1;
+          }
         }
+        mma_commit_leader(leader, &S.o_done[u & 1]);
         if (__any_sync(kAll, cp.last())) ++on;
+        done_pv += two ? 2 : 1;
         cp.advance(a, x_begin, x_end);
         return true;
       };
-      // PV(g) goes out before S(g + 2).  The wait for P(g) says that the softmax has read S(g) and the tile's scales, so
-      // S's buffer is free; and as MMAs complete in order, a softmax that sees S(g + 2) knows that PV(g) has read P's.
+      // PV of pair u goes out before S of pair u + 2.  The wait for P(u) says that the softmax has read S(u) and the tiles'
+      // scales, so S's buffer is free; and as MMAs complete in order, a softmax that sees S(u + 2) knows that PV(u) has
+      // read P's.
       bool ok = issue_s(0);
-      if (ok && count > 1) ok = issue_s(1);
-      for (int g = 0; g < count && ok; ++g) {
-        ok = issue_pv(g);
-        if (ok && g + 2 < count) ok = issue_s(g + 2);
+      if (ok && done_s < count) ok = issue_s(1);
+      for (int u = 0; ok && done_pv < count; ++u) {
+        ok = issue_pv(u);
+        if (ok && done_s < count) ok = issue_s(u + 2);
       }
     }
   } else if (warp >= kQueryWarp) {
@@ -403,10 +451,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         reinterpret_cast<uint4*>(a.out + (long long)(r.q_start + i / chunks) * a.out_row_stride)[i % chunks] =
             make_uint4(0u, 0u, 0u, 0u);
     }
-  } else if (warp >= kSoftmaxWarp && ntiles > 0) {
+  } else if (softmax) {
+    registers_up<kSoftmaxRegs>();
     // ------------------------------------------------------------------ softmax / correction / epilogue
     const int wg = (warp - kSoftmaxWarp) >> 2;   // column group: columns cb .. cb + 15
-    const int cb = wg * kGroupCols;
+    const int cb = wg * kGroupCols, p0 = cb / G; // and its first query position (G divides 16)
     const int w = warp & 3;                      // TMEM lane quadrant
     const int row = (threadIdx.x - kSoftmaxWarp * 32) & 127;   // key within the tile (S^T) / head dim (O^T)
     const int col = cb + (lane & 15);            // the column that lane j (and j + 16) speaks for
@@ -417,9 +466,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int c = blockIdx.x;
     const int my_group = row / a.group;
     Walk<QMAX, true> wk;
-    wk.start(a, S);
-    bool ok = true;
-    int g = 0;
+    bool ok = ntiles > 0;
+    if (ok) wk.start(a, S);
+    int g = 0, u = 0;              // tiles and pairs handed over
     for (int n = 0; ok && wk.A < x_end; wk.next(a), ++n) {
       const int L = wk.r.L, ql = wk.r.ql;
       const int t0 = wk.t0(x_begin), t1 = wk.t1(x_end);
@@ -440,51 +489,70 @@ __global__ void __launch_bounds__(kThreads, 1)
         m_neg[j] = -kNegBig;
         l_part[j] = 0.0f;
       }
-      for (int t = t0; t < t1; ++t, ++g) {
-        const int buf = g & 1;
-        if (!mbar_wait(&S.s_full[buf], (g >> 1) & 1, abort, a.err, kErrTimeoutS)) { ok = false; break; }
+      for (int t = t0; t < t1; t += 2, ++u) {
+        const bool two = t + 1 < t1;
+        const int buf = u & 1;
+        if (!mbar_wait(&S.s_full[buf], (u >> 1) & 1, abort, a.err, kErrTimeoutS)) { ok = false; break; }
         tc_fence_after();
-        const int key = t * kKeysPerTile + row;
         if (live) {
           if (t == t0) q_factor = S.q_scale[n & 3] * a.scale_log2;
-          const int e = g % kScaleStages;
-          const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
-          float x[kGroupCols], x2[kGroupCols];
-          const uint32_t tmem_s = tmem + lane_off + buf * 64 + cb;
-          tmem_ld_32x32b_2x16(tmem_s, tmem_s + kCols, x, x2);
-          const float log_vs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
-          const float factor = ks * q_factor;
+          // distances of both tiles' t = score + log2 vs from the running maxima (a missing second tile: nothing)
+          float d[2][kGroupCols], inv_vs[2];
+          {
+            uint32_t r[2][16], r2[2][16];
+            const uint32_t tmem_s = tmem + lane_off + buf * kTmemSPair + cb;
+            tmem_ld_start_2x16(tmem_s, tmem_s + kCols, r[0], r2[0]);
+            if (two) tmem_ld_start_2x16(tmem_s + kTmemSTile, tmem_s + kTmemSTile + kCols, r[1], r2[1]);
+            float factor[2], log_vs[2];
 #pragma unroll
-          for (int j = 0; j < kGroupCols; j += 2) {
-            const float2 s = fma_x2(make_float2(x2[j], x2[j + 1]), make_float2(0.0625f, 0.0625f), make_float2(x[j], x[j + 1]));
-            const float2 t2 = fma_x2(s, make_float2(factor, factor), make_float2(log_vs, log_vs));
-            x[j] = t2.x;
-            x[j + 1] = t2.y;
-          }
-          if ((t * kKeysPerTile + kKeysPerTile - 1) > min_limit) {
-#pragma unroll
-            for (int j = 0; j < kGroupCols; ++j) {
-              const int p = (cb + j) / G;
-              const int limit = (a.causal && p < ql) ? L - ql + p : L - 1;
-              x[j] = key <= limit ? x[j] : -INFINITY;
+            for (int i = 0; i < 2; ++i) {
+              const int e = (g + i) % kScaleStages;
+              const float ks = S.scales[e][0][my_group], vs = fmaxf(S.scales[e][1][my_group], kMinScale);
+              factor[i] = ks * q_factor;
+              log_vs[i] = __log2f(vs);
+              inv_vs[i] = __fdividef(1.0f, vs);
             }
+            tmem_ld_wait_2x16(r[0], r2[0]);
+            tmem_ld_wait_2x16(r[1], r2[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < kGroupCols; j += 2) {
+                const float2 s2 = fma_x2(make_float2(__uint_as_float(r2[i][j]), __uint_as_float(r2[i][j + 1])),
+                                         make_float2(0.0625f, 0.0625f),
+                                         make_float2(__uint_as_float(r[i][j]), __uint_as_float(r[i][j + 1])));
+                const float2 t2 = fma_x2(s2, make_float2(factor[i], factor[i]), make_float2(log_vs[i], log_vs[i]));
+                d[i][j] = t2.x;
+                d[i][j + 1] = t2.y;
+              }
+          }
+          if ((t + 2) * kKeysPerTile - 1 > min_limit) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int key = (t + i) * kKeysPerTile + row;
+#pragma unroll
+              for (int j = 0; j < kGroupCols; ++j) {
+                const int p = p0 + j / G;
+                const int limit = (a.causal && p < ql) ? L - ql + p : L - 1;
+                d[i][j] = key <= limit && (i == 0 || two) ? d[i][j] : -INFINITY;
+              }
+            }
+          } else if (!two) {         // the piece's last tile, its item going on in another CTA
+#pragma unroll
+            for (int j = 0; j < kGroupCols; ++j) d[1][j] = -INFINITY;
           }
           // ---- does any score of the group pass its column's running maximum by more than 2^8?  Only then (always at an
-          // item's first tile) are the tile's column maxima taken: this warp's, then the four warps'
-          float over = -INFINITY, d[kGroupCols];
-          __half2 ph[kGroupCols / 2];
+          // item's first pair) are the pair's column maxima taken: this warp's, then the four warps'
+          float over = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < kGroupCols; j += 2) {
-            const float2 d2 = add_x2(make_float2(x[j], x[j + 1]), make_float2(m_neg[j], m_neg[j + 1]));
-            d[j] = d2.x;
-            d[j + 1] = d2.y;
-            over = fmaxf(fmaxf(over, d2.x), d2.y);
-          }
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < kGroupCols; ++j) over = fmaxf(over, d[i][j] + m_neg[j]);
           if (named_barrier_or(bar_wg, 128, over > 8.0f + kPBias)) {
             float wmax = -INFINITY;
 #pragma unroll
             for (int j = 0; j < kGroupCols; ++j) {
-              const float v = warp_max_redux(x[j]);
+              const float v = warp_max_redux(fmaxf(d[0][j], d[1][j]));
               wmax = lane == j ? v : wmax;
             }
             if (lane < kGroupCols) S.red_max[buf][col][w] = wmax;
@@ -494,67 +562,71 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float m_new = tmax > m_lane + 8.0f ? tmax : m_lane;
             const float alpha_lane = ex2_approx(m_lane - m_new);
             m_lane = m_new;
-            float alpha[kGroupCols];
 #pragma unroll
-            for (int j = 0; j < kGroupCols; ++j) {
-              alpha[j] = __shfl_sync(0xffffffffu, alpha_lane, j);
-              m_neg[j] = kPBias - __shfl_sync(0xffffffffu, m_new, j);
-              l_part[j] *= alpha[j];
-              d[j] = x[j] + m_neg[j];
-            }
-            if (t > t0) {     // O holds this item's earlier tiles: rescale its parts once PV(g-1) has landed
-              if (!mbar_wait(&S.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
+            for (int j = 0; j < kGroupCols; ++j) m_neg[j] = kPBias - __shfl_sync(0xffffffffu, m_new, j);
+            if (t > t0) {     // O holds this item's earlier tiles: rescale its parts once the last PV has landed
+#pragma unroll
+              for (int j = 0; j < kGroupCols; ++j) l_part[j] *= __shfl_sync(0xffffffffu, alpha_lane, j);
+              if (!mbar_wait(&S.o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) { ok = false; break; }
               tc_fence_after();
 #pragma unroll 1
               for (int part = 0; part < kPParts; ++part) {
                 float o[kGroupCols];
                 tmem_ld_32x32b_x16(tmem_o + part * kCols, o);
 #pragma unroll
-                for (int j = 0; j < kGroupCols; ++j) o[j] *= alpha[j];
+                for (int j = 0; j < kGroupCols; ++j) o[j] *= __shfl_sync(0xffffffffu, alpha_lane, j);
                 tmem_st_32x32b_x16(tmem_o + part * kCols, o);
               }
             }
           }
+          // ---- probabilities, column sums, and this group's 16 columns of row `row` of the parts (S(u) seen: PV(u-2) has
+          // released the buffer).  An fp16 pattern's high byte is its value cut to e5m2; what is left over is exact in
+          // fp16.  Two cuts, then the third part to nearest: fp16's 2^-12 and e5m2's last half step, 2^-9 of p', off it.
 #pragma unroll
-          for (int j = 0; j < kGroupCols; j += 2) {
-            const float2 p2 = make_float2(ex2_approx(d[j]), ex2_approx(d[j + 1]));      // masked: 0
-            const float2 l2 = fma_x2(p2, make_float2(inv_vs, inv_vs), make_float2(l_part[j], l_part[j + 1]));
-            l_part[j] = l2.x;
-            l_part[j + 1] = l2.y;
-            ph[j / 2] = __floats2half2_rn(p2.x, p2.y);
-          }
-          // ---- this group's 16 columns of row `row` of the three parts (S(g) seen: PV(g-2) has released the buffer)
-          // An fp16 pattern's high byte is its value cut to e5m2; what is left over is exact in fp16.  Two cuts, then the
-          // third part to nearest: p is fp16's 2^-12 and e5m2's last half step, 2^-9 of p, from p'.
-          unsigned char* prow = sP + buf * kPBytes + row * kCols + (wg ^ ((row >> 2) & 1)) * 16;
+          for (int i = 0; i < 2; ++i) {
+            if (i == 1 && !two) break;
+            __half2 ph[kGroupCols / 2];
 #pragma unroll
-          for (int part = 0; part < kPParts; ++part) {
-            unsigned wd[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              unsigned lo = half2_bits(ph[2 * k]), hi = half2_bits(ph[2 * k + 1]);
-              if (part == kPParts - 1) {
-                lo += 0x00800080u;
-                hi += 0x00800080u;
-              } else {
-                ph[2 * k] = __hsub2(ph[2 * k], bits_half2(lo & 0xff00ff00u));
-                ph[2 * k + 1] = __hsub2(ph[2 * k + 1], bits_half2(hi & 0xff00ff00u));
-              }
-              wd[k] = __byte_perm(lo, hi, 0x7531);
+            for (int j = 0; j < kGroupCols; j += 2) {
+              const float2 d2 = add_x2(make_float2(d[i][j], d[i][j + 1]), make_float2(m_neg[j], m_neg[j + 1]));
+              const float2 p2 = make_float2(ex2_approx(d2.x), ex2_approx(d2.y));      // masked: 0
+              const float2 l2 = fma_x2(p2, make_float2(inv_vs[i], inv_vs[i]), make_float2(l_part[j], l_part[j + 1]));
+              l_part[j] = l2.x;
+              l_part[j + 1] = l2.y;
+              ph[j / 2] = __floats2half2_rn(p2.x, p2.y);
             }
-            *reinterpret_cast<uint4*>(prow + part * kPPartBytes) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+            unsigned char* prow = sP + (buf * 2 + i) * kPBytes + row * kCols + (wg ^ ((row >> 2) & 1)) * 16;
+#pragma unroll
+            for (int part = 0; part < kPParts; ++part) {
+              unsigned wd[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                unsigned lo = half2_bits(ph[2 * k]), hi = half2_bits(ph[2 * k + 1]);
+                if (part == kPParts - 1) {
+                  lo += 0x00800080u;
+                  hi += 0x00800080u;
+                } else {
+                  ph[2 * k] = __hsub2(ph[2 * k], bits_half2(lo & 0xff00ff00u));
+                  ph[2 * k + 1] = __hsub2(ph[2 * k + 1], bits_half2(hi & 0xff00ff00u));
+                }
+                wd[k] = __byte_perm(lo, hi, 0x7531);
+              }
+              *reinterpret_cast<uint4*>(prow + part * kPPartBytes) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+            }
           }
         }
+        const int last = two ? 1 : 0;
         // ---- the row's last tile: V rows past the context are zeroed; each group zeroes half of the row
-        if ((t + 1) * kKeysPerTile > L) {
-          const int stage = g % kStages;
-          if (!mbar_wait(&S.v_full[stage], (g / kStages) & 1, abort, a.err, kErrTimeoutV)) { ok = false; break; }
-          if (key >= L) {
+        if ((t + last + 1) * kKeysPerTile > L) {
+          const int gl = g + last, stage = gl % kStages;
+          if (!mbar_wait(&S.v_full[stage], (gl / kStages) & 1, abort, a.err, kErrTimeoutV)) { ok = false; break; }
+          if ((t + last) * kKeysPerTile + row >= L) {
             unsigned char* v0 = sV + stage * kTileBytes + row * kHeadDim + wg * 64;
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc) *reinterpret_cast<uint4*>(v0 + cc * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
+        g += last + 1;
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
@@ -567,8 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < kGroupCols) S.red_sum[col][w] = s;
       }
       named_barrier(bar_wg, 128);
-      const int gl = g - 1;
-      if (!mbar_wait(&S.o_done[gl & 1], (gl >> 1) & 1, abort, a.err, kErrTimeoutO)) break;
+      if (!mbar_wait(&S.o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort, a.err, kErrTimeoutO)) break;
       tc_fence_after();
       float o[kGroupCols];
       {
@@ -656,14 +727,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!live) continue;
       const float inv_lane = l_lane > 0.0f ? 1.0f / l_lane : l_lane;      // nothing seen: 0 (and NaN stays)
-      const int d = row;
+      __nv_bfloat16* dst = a.out + (long long)(wk.r.q_start + p0) * a.out_row_stride + wk.h * (G * kHeadDim) + row;
 #pragma unroll
       for (int j = 0; j < kGroupCols; ++j) {
-        const int p = (cb + j) / G, gq = (cb + j) % G;
         const float inv = __shfl_sync(0xffffffffu, inv_lane, j);
-        if (p < ql)
-          a.out[(long long)(wk.r.q_start + p) * a.out_row_stride + (long long)(wk.h * G + gq) * kHeadDim + d] =
-              __float2bfloat16_rn(o[j] * inv);
+        if (p0 + j / G < ql) dst[(j / G) * a.out_row_stride + (j % G) * kHeadDim] = __float2bfloat16_rn(o[j] * inv);
       }
     }
   }
@@ -693,6 +761,12 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t block_size, uin
 template <int G>
 static int launch(const CUtensorMap (&m)[4], const Args& a, int grid, bool early, cudaStream_t stream) {
   if (int st = ensure_dynamic_smem<verify_attention_fp8_kernel<G>>(kSmemBytes)) return st;
+  static const int regs = [] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, verify_attention_fp8_kernel<G>) == cudaSuccess ? attr.numRegs : -1;
+  }();
+  if (regs < kLaunchRegs)      // the register shares would wait for registers that the block does not have
+    return set_error(kCudaError, "attention built with %d registers a thread, %d needed", regs, kLaunchRegs);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kThreads);

@@ -156,6 +156,32 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
     return device
 
 
+def same_device(index: int, *tensors: torch.Tensor | None) -> bool:
+    """Whether index is a CUDA device's and every given tensor is on it (require_cuda names the one that is not)."""
+    if index < 0:
+        return False
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != index:
+            return False
+    return True
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of CUDA device `index`, as its address: stream_of without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def call_on(index: int, function, *args) -> None:
+    """A library call with device `index` current (the library takes sizes and launches on the current device)."""
+    if torch._C._cuda_getDevice() == index:
+        status = function(*args)
+    else:
+        with torch.cuda.device(index):
+            status = function(*args)
+    if status != 0:
+        check(status)
+
+
 class Workspace:
     """A zero-initialised device byte buffer per (device, name), grown on demand.  The library keeps its tickets
     and argmax keys self-cleaning at fixed offsets, so the buffer is zeroed once per allocation only.  A grown
@@ -164,6 +190,14 @@ class Workspace:
 
     _buffers: dict[tuple[int, str], torch.Tensor] = {}
     _retired: list[torch.Tensor] = []
+
+    @classmethod
+    def address(cls, index: int, nbytes: int, name: str) -> int:
+        """The address of the buffer get(cuda:index, nbytes, name) returns."""
+        buf = cls._buffers.get((index, name))
+        if buf is None or buf.numel() < nbytes:
+            buf = cls.get(torch.device("cuda", index), nbytes, name)
+        return buf.data_ptr()
 
     @classmethod
     def get(cls, device: torch.device, nbytes: int, name: str = "sampler") -> torch.Tensor:

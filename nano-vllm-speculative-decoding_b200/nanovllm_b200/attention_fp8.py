@@ -30,12 +30,13 @@ the cache, 5 a block id outside the cache (read as block 0).
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
 from . import _lib
-from ._lib import check, ptr, require_cuda, stream_of
-from .attention import CTAS_SHIFT, EARLY_LAUNCH, _err_word, _output, _row_metadata, _split_workspace
+from ._lib import Workspace, call_on, ptr, raw_stream, require_cuda, same_device
+from .attention import _SPLIT_MIN_BYTES, CTAS_SHIFT, EARLY_LAUNCH, _output
 from .context import get_context
 
 HEAD_DIM = 128
@@ -76,45 +77,64 @@ class FP8Cache:
 
 def _cache_geometry(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
     """(blocks, Hkv, block_size, group) of a checked cache."""
-    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+    if k_cache.dtype is not torch.float8_e4m3fn or v_cache.dtype is not torch.float8_e4m3fn:
         raise ValueError(f"the 8-bit caches are float8_e4m3fn (got {k_cache.dtype}, {v_cache.dtype})")
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
         raise ValueError("the scales are float32")
-    if k_cache.dim() != 4 or k_cache.shape[3] != HEAD_DIM or v_cache.shape != k_cache.shape:
+    shape, scale_shape = tuple(k_cache.shape), tuple(k_scale.shape)
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v_cache.shape != shape:
         raise ValueError(f"caches must be [blocks, Hkv, block_size, {HEAD_DIM}] of one shape "
-                         f"(got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
-    blocks, kv_heads, block_size, _ = k_cache.shape
-    if (k_scale.dim() != 3 or v_scale.shape != k_scale.shape or k_scale.shape[:2] != (blocks, kv_heads)
-            or k_scale.shape[2] * 16 not in (block_size, block_size // 2)):
+                         f"(got {shape}, {tuple(v_cache.shape)})")
+    blocks, kv_heads, block_size, _ = shape
+    if (len(scale_shape) != 3 or v_scale.shape != scale_shape or scale_shape[:2] != shape[:2]
+            or (scale_shape[2] * 16 != block_size and scale_shape[2] * 32 != block_size)):
         raise ValueError(f"scales must be [blocks, Hkv, block_size / 16 or / 32] of one shape "
-                         f"(got {tuple(k_scale.shape)}, {tuple(v_scale.shape)} for caches {tuple(k_cache.shape)})")
-    if not all(t.is_contiguous() for t in (k_cache, v_cache, k_scale, v_scale)):
+                         f"(got {scale_shape}, {tuple(v_scale.shape)} for caches {shape})")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
         raise ValueError("caches and scales must be contiguous")
-    return blocks, kv_heads, block_size, block_size // k_scale.shape[2]
+    return blocks, kv_heads, block_size, block_size // scale_shape[2]
+
+
+def _int32(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t as a contiguous int32 tensor (itself where it is one)."""
+    if t is None or (t.dtype is torch.int32 and t.is_contiguous()):
+        return t
+    return t.to(torch.int32).contiguous()
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(index: int, R: int, kv_heads: int) -> int:
+    with torch.cuda.device(index):
+        need = int(_lib.lib().specdec_attention_workspace_bytes(R, kv_heads))
+    if need < 0:
+        raise _lib.SpecdecError(f"no attention workspace for {R} rows of {kv_heads} KV heads")
+    return max(need, _SPLIT_MIN_BYTES)
 
 
 def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """key / value [N, Hkv, 128] bf16 rows (dense heads, rows may be strided) to slot_mapping [N] of the 8-bit caches,
     in any order; slot -1 skipped.  At most 16384 tokens a call."""
-    device = require_cuda(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    index = key.get_device()
+    if not same_device(index, value, k_cache, v_cache, k_scale, v_scale, slot_mapping):
+        require_cuda(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     blocks, kv_heads, block_size, group = _cache_geometry(k_cache, v_cache, k_scale, v_scale)
-    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+    if key.dtype is not torch.bfloat16 or value.dtype is not torch.bfloat16:
         raise ValueError("the B200 K/V store takes bf16 keys and values")
-    if key.dim() != 3 or key.shape[1:] != (kv_heads, HEAD_DIM) or value.shape != key.shape:
-        raise ValueError(f"key and value must be [N, {kv_heads}, {HEAD_DIM}] (got {tuple(key.shape)}, "
-                         f"{tuple(value.shape)})")
-    N = key.shape[0]
-    for t in (key, value):
-        if N and (t.stride(2) != 1 or (kv_heads > 1 and t.stride(1) != HEAD_DIM)):
-            raise ValueError("key and value rows must hold their heads densely")
+    shape = tuple(key.shape)
+    if len(shape) != 3 or shape[1:] != (kv_heads, HEAD_DIM) or value.shape != shape:
+        raise ValueError(f"key and value must be [N, {kv_heads}, {HEAD_DIM}] (got {shape}, {tuple(value.shape)})")
+    N = shape[0]
+    ks, vs = key.stride(), value.stride()
+    if N and (ks[2] != 1 or vs[2] != 1 or (kv_heads > 1 and (ks[1] != HEAD_DIM or vs[1] != HEAD_DIM))):
+        raise ValueError("key and value rows must hold their heads densely")
     if slot_mapping.numel() != N:
         raise ValueError(f"{slot_mapping.numel()} slots for {N} tokens")
-    slots = slot_mapping.to(torch.int32).contiguous()
-    with torch.cuda.device(device):
-        check(_lib.lib().specdec_store_kvcache_fp8(
-            ptr(key), key.stride(0), ptr(value), value.stride(0), ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale),
-            ptr(slots), N, kv_heads, HEAD_DIM, blocks, block_size, group, ptr(_err_word(device)), stream_of(device)))
+    slots = _int32(slot_mapping)
+    call_on(index, _lib.lib().specdec_store_kvcache_fp8, key.data_ptr(), ks[0], value.data_ptr(), vs[0],
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), N, kv_heads,
+            HEAD_DIM, blocks, block_size, group, Workspace.address(index, 256, "attention"), raw_stream(index))
 
 
 def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -127,30 +147,43 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     """attention.paged_attention over the 8-bit caches: q [T, H, 128] bf16, varlen (cu_seqlens_q/k, max_seqlen_q) or
     decode (context_lens with query_len_per_seq queries a row).  Returns out [T, H, 128] bf16; rows of out behind the last
     sequence are left as they were.  early_launch, max_ctas and workspace as there."""
-    device = require_cuda(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_q, cu_seqlens_k, context_lens)
+    index = q.get_device()
+    if not same_device(index, k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_q, cu_seqlens_k, context_lens):
+        require_cuda(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_q, cu_seqlens_k, context_lens)
     blocks, kv_heads, block_size, group = _cache_geometry(k_cache, v_cache, k_scale, v_scale)
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != HEAD_DIM:
-        raise ValueError(f"q must be bf16 [T, H, {HEAD_DIM}] (got {q.dtype} {tuple(q.shape)})")
-    if cu_seqlens_q is None and context_lens is None:
+    shape = tuple(q.shape)
+    if q.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM:
+        raise ValueError(f"q must be bf16 [T, H, {HEAD_DIM}] (got {q.dtype} {shape})")
+    T, H, D = shape
+    if cu_seqlens_q is not None:
+        if cu_seqlens_k is None or max_seqlen_q is None:
+            raise ValueError("varlen attention needs cu_seqlens_k and max_seqlen_q")
+        cq, ck, ctx = _int32(cu_seqlens_q), _int32(cu_seqlens_k), None
+        R, q_per_seq, max_q = cq.numel() - 1, 0, int(max_seqlen_q)
+        if ck.numel() != R + 1:
+            raise ValueError(f"cu_seqlens_q of {R} rows, cu_seqlens_k of {ck.numel() - 1}")
+    elif context_lens is not None:
+        cq, ck, ctx = None, None, _int32(context_lens)
+        R, q_per_seq, max_q = ctx.numel(), query_len_per_seq, query_len_per_seq
+    else:
         raise ValueError("give cu_seqlens_q / cu_seqlens_k (varlen) or context_lens (decode)")
+    tables = _int32(block_tables)
+    if tables.dim() != 2 or tables.shape[0] != R:
+        raise ValueError(f"block tables {tuple(tables.shape)} for {R} rows")
     if not 0 <= max_ctas <= 255:
         raise ValueError(f"max_ctas {max_ctas}: 0 (one CTA per SM) to 255")
-    T, H, D = q.shape
-    out = _output(out, q.shape, device)
-    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _output(out, shape, q.device)
+    strides = q.stride()
+    if strides[2] != 1 or strides[1] != D or strides[0] % 8 or q.data_ptr() % 16:
         q = q.contiguous()
-    tables, cq, ck, ctx, R, q_per_seq, max_q = _row_metadata(block_tables, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
-                                                              context_lens, query_len_per_seq)
-    if tables.dim() != 2 or tables.shape[0] != R or (ck is not None and ck.numel() != R + 1):
-        raise ValueError(f"block tables {tuple(tables.shape)} and lengths disagree on the {R} rows")
-    ws = _split_workspace(device, R, kv_heads, workspace)
+        strides = q.stride()
+    ws_bytes = _workspace_bytes(index, R, kv_heads)
     flags = (EARLY_LAUNCH if early_launch else 0) | (max_ctas << CTAS_SHIFT)
-    with torch.cuda.device(device):
-        check(_lib.lib().specdec_paged_attention_fp8(
-            ptr(q), T, q.stride(0), H, kv_heads, D, ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), blocks,
-            block_size, group, ptr(cq), ptr(ck), ptr(ctx), q_per_seq, R, ptr(tables), tables.shape[1], max_q, float(scale),
-            int(causal), ptr(out), out.stride(0), ptr(ws), ws.numel(), ptr(_err_word(device)), flags,
-            stream_of(device)))
+    call_on(index, _lib.lib().specdec_paged_attention_fp8, q.data_ptr(), T, strides[0], H, kv_heads, D,
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size, group,
+            ptr(cq), ptr(ck), ptr(ctx), q_per_seq, R, tables.data_ptr(), tables.shape[1], max_q, scale, causal,
+            out.data_ptr(), out.stride(0), Workspace.address(index, ws_bytes, workspace), ws_bytes,
+            Workspace.address(index, 256, "attention"), flags, raw_stream(index))
     return out
 
 

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import Workspace, check, ptr, require_cuda, stream_of
+from ._lib import Workspace, call_on, ptr, raw_stream, require_cuda, same_device
 from .batch_metadata import packed_sizes
 
 
@@ -34,11 +34,9 @@ def reset_device_error(device: torch.device) -> None:
     _words(device)[0].zero_()
 
 
-def _of(name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor | None:
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {device} (got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device})")
-    return t
+def _of(name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple) -> None:
+    if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} (got {t.dtype} {tuple(t.shape)})")
 
 
 def verify_metadata(lengths: torch.Tensor, last_tokens: torch.Tensor, drafts: torch.Tensor,
@@ -55,31 +53,34 @@ def verify_metadata(lengths: torch.Tensor, last_tokens: torch.Tensor, drafts: to
     free_blocks[:free_count] (int32, free_count [1] int32, lowered in place), rows in order.  Both None: the rows must
     hold what they need.  The row arguments may be empty (R = 0): all padding.  Calls on one device share an error word and
     a ticket: they must not overlap on the GPU."""
-    device = require_cuda(lengths, last_tokens, drafts, verified_lens, block_tables, num_blocks, free_blocks, free_count,
-                          buf64, buf32)
+    index = buf64.get_device()
+    if not same_device(index, lengths, last_tokens, drafts, verified_lens, block_tables, num_blocks, free_blocks,
+                       free_count, buf32):
+        require_cuda(buf64, lengths, last_tokens, drafts, verified_lens, block_tables, num_blocks, free_blocks, free_count,
+                     buf32)
     if drafts.dim() != 2 or block_tables.dim() != 2:
         raise ValueError("drafts and block_tables must be 2-D")
     R, k = drafts.shape
-    _of("lengths", lengths, torch.int64, (R,), device)
-    _of("last_tokens", last_tokens, torch.int64, (R,), device)
-    _of("drafts", drafts, torch.int64, (R, k), device)
-    _of("verified_lens", verified_lens, torch.int64, (R,), device)
-    _of("block_tables", block_tables, torch.int32, (R, block_tables.shape[1]), device)
-    _of("num_blocks", num_blocks, torch.int32, (R,), device)
+    table_width = block_tables.shape[1]
+    rows = (R,)
+    _of("lengths", lengths, torch.int64, rows)
+    _of("last_tokens", last_tokens, torch.int64, rows)
+    _of("drafts", drafts, torch.int64, (R, k))
+    _of("verified_lens", verified_lens, torch.int64, rows)
+    _of("block_tables", block_tables, torch.int32, (R, table_width))
+    _of("num_blocks", num_blocks, torch.int32, rows)
     if (free_blocks is None) != (free_count is None):
         raise ValueError("give free_blocks and free_count together")
     capacity = 0
     if free_blocks is not None:
         capacity = free_blocks.numel()
-        _of("free_blocks", free_blocks, torch.int32, (capacity,), device)
-        _of("free_count", free_count, torch.int32, (1,), device)
+        _of("free_blocks", free_blocks, torch.int32, (capacity,))
+        _of("free_count", free_count, torch.int32, (1,))
     n64, n32 = packed_sizes(num_rows, num_tokens, width)
-    _of("buf64", buf64, torch.int64, (n64,), device)
-    _of("buf32", buf32, torch.int32, (n32,), device)
-    words = _words(device)
-    with torch.cuda.device(device):
-        check(_lib.lib().specdec_verify_metadata(
-            ptr(lengths), ptr(last_tokens), ptr(drafts), ptr(verified_lens), R, k, ptr(block_tables),
-            block_tables.shape[1], ptr(num_blocks), ptr(free_blocks), ptr(free_count), capacity, block_size, num_rows,
-            num_tokens, pad_block_id, width, ptr(buf64), ptr(buf32), words.data_ptr() + 4, words.data_ptr(),
-            stream_of(device)))
+    _of("buf64", buf64, torch.int64, (n64,))
+    _of("buf32", buf32, torch.int32, (n32,))
+    words = Workspace.address(index, 256, "device_metadata")       # [error word, ticket]
+    call_on(index, _lib.lib().specdec_verify_metadata, ptr(lengths), ptr(last_tokens), ptr(drafts), ptr(verified_lens), R,
+            k, ptr(block_tables), table_width, ptr(num_blocks), ptr(free_blocks), ptr(free_count), capacity, block_size,
+            num_rows, num_tokens, pad_block_id, width, buf64.data_ptr(), buf32.data_ptr(), words + 4, words,
+            raw_stream(index))

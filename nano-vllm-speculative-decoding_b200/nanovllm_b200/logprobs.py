@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODES, Workspace, check, ptr, require_cuda, stream_of
+from ._lib import DTYPE_CODES, Workspace, call_on, ptr, raw_stream, require_cuda, same_device
 
 MAX_TOP = 32
 
@@ -46,7 +46,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, num_top: int = 0,
     index, NaN above every number.  Rows whose token is negative (padding) are not read: 0, 0, ids -1, 0.  A row with a
     NaN or +inf, or nothing but -inf, has NaN for every log probability and the entropy; a single -inf is a token of
     probability 0."""
-    device = require_cuda(logits, tokens, temperatures)
+    index = logits.get_device()
+    if not same_device(index, tokens, temperatures):
+        require_cuda(logits, tokens, temperatures)
     if logits.dim() != 2 or logits.dtype not in DTYPE_CODES:
         raise ValueError(f"logits must be [T, V] bf16, fp16 or fp32 (got {logits.dtype} {tuple(logits.shape)})")
     T, V = logits.shape
@@ -63,14 +65,14 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, num_top: int = 0,
     if T and (logits.stride(1) != 1 or (T > 1 and logits.stride(0) < V)):
         logits = logits.contiguous()
     stride = logits.stride(0) if T > 1 else V
-    tokens = tokens.to(torch.int64).contiguous()
-    out = TokenLogprobs(torch.empty(T, dtype=torch.float32, device=device),
-                        torch.empty(T, dtype=torch.float32, device=device),
-                        torch.empty(T, num_top, dtype=torch.int64, device=device),
-                        torch.empty(T, num_top, dtype=torch.float32, device=device))
-    with torch.cuda.device(device):
-        check(_lib.lib().specdec_token_logprobs(
-            ptr(logits), DTYPE_CODES[logits.dtype], T, V, stride, ptr(tokens), ptr(temperatures), num_top,
-            ptr(out.logprobs), ptr(out.entropy), ptr(out.top_ids), ptr(out.top_logprobs), ptr(_err_word(device)),
-            stream_of(device)))
+    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    device = logits.device
+    floats = torch.empty(T * (2 + num_top), dtype=torch.float32, device=device)      # one allocation for the three
+    out = TokenLogprobs(floats[:T], floats[T:2 * T], torch.empty(T, num_top, dtype=torch.int64, device=device),
+                        floats[2 * T:].view(T, num_top))
+    base = floats.data_ptr()
+    call_on(index, _lib.lib().specdec_token_logprobs, logits.data_ptr(), DTYPE_CODES[logits.dtype], T, V, stride,
+            tokens.data_ptr(), ptr(temperatures), num_top, base, base + 4 * T, out.top_ids.data_ptr(), base + 8 * T,
+            Workspace.address(index, 256, "logprobs"), raw_stream(index))
     return out

@@ -313,10 +313,14 @@ int specdec_verify_metadata(const long long* lengths, const long long* last_toke
  * T * V probabilities): for each row of logits [T][V] (dtype code, row stride in elements) divided by temperatures [T]
  * (null: 1), logprobs[t] = log softmax at tokens[t], entropy[t] in nats, and the num_top (0 .. 32) largest logits' ids
  * (ties to the lowest index, NaN above all) and log probabilities [T][num_top].  A negative token: the row is not read,
- * 0, 0, ids -1, 0.  A token past V: NaN and *err = 8.  T <= 65535, V <= 2^24. */
+ * 0, 0, ids -1, 0.  A token past V: NaN and *err = 8.  T <= 65535, V <= 2^24.  workspace: 256-byte aligned device bytes,
+ * zero-filled once before first use (the kernel leaves its tickets zeroed), at least
+ * specdec_logprobs_workspace_bytes(T, V, dtype, num_top); calls sharing it must not overlap on the GPU. */
+long long specdec_logprobs_workspace_bytes(long long T, long long V, int dtype, int num_top);
 int specdec_token_logprobs(const void* logits, int dtype, long long T, long long V, long long row_stride,
                            const long long* tokens, const float* temperatures, int num_top, float* logprobs,
-                           float* entropy, long long* top_ids, float* top_logprobs, int* err, void* stream);
+                           float* entropy, long long* top_ids, float* top_logprobs, void* workspace,
+                           long long workspace_bytes, int* err, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -8,6 +8,7 @@ probabilities wants a few numbers for each emitted token.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -39,13 +40,20 @@ def reset_device_error(device: torch.device) -> None:
     _err_word(device).zero_()
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(index: int, T: int, V: int, dtype: int, num_top: int) -> int:
+    with torch.cuda.device(index):
+        return int(_lib.lib().specdec_logprobs_workspace_bytes(T, V, dtype, num_top))
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, num_top: int = 0,
-                   temperatures: torch.Tensor | None = None) -> TokenLogprobs:
+                   temperatures: torch.Tensor | None = None, *, workspace: str = "logprobs_parts") -> TokenLogprobs:
     """logits [T, V] (bf16, fp16 or fp32; rows may be strided), tokens [T] int64.  temperatures [T] fp32 > 0 (None: 1)
     divide the logits first.  num_top (0 to 32, at most V) alternatives a row: the largest logits, ties to the lowest
     index, NaN above every number.  Rows whose token is negative (padding) are not read: 0, 0, ids -1, 0.  A row with a
     NaN or +inf, or nothing but -inf, has NaN for every log probability and the entropy; a single -inf is a token of
-    probability 0."""
+    probability 0.  workspace: the name of the device workspace; calls that may run at the same time on different streams
+    need different names."""
     index = logits.get_device()
     if not same_device(index, tokens, temperatures):
         require_cuda(logits, tokens, temperatures)
@@ -71,8 +79,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, num_top: int = 0,
     floats = torch.empty(T * (2 + num_top), dtype=torch.float32, device=device)      # one allocation for the three
     out = TokenLogprobs(floats[:T], floats[T:2 * T], torch.empty(T, num_top, dtype=torch.int64, device=device),
                         floats[2 * T:].view(T, num_top))
-    base = floats.data_ptr()
-    call_on(index, _lib.lib().specdec_token_logprobs, logits.data_ptr(), DTYPE_CODES[logits.dtype], T, V, stride,
-            tokens.data_ptr(), ptr(temperatures), num_top, base, base + 4 * T, out.top_ids.data_ptr(), base + 8 * T,
-            Workspace.address(index, 256, "logprobs"), raw_stream(index))
+    base, dtype = floats.data_ptr(), DTYPE_CODES[logits.dtype]
+    ws_bytes = _workspace_bytes(index, T, V, dtype, num_top)
+    call_on(index, _lib.lib().specdec_token_logprobs, logits.data_ptr(), dtype, T, V, stride, tokens.data_ptr(),
+            ptr(temperatures), num_top, base, base + 4 * T, out.top_ids.data_ptr(), base + 8 * T,
+            Workspace.address(index, ws_bytes, workspace), ws_bytes, Workspace.address(index, 256, "logprobs"),
+            raw_stream(index))
     return out

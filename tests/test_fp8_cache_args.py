@@ -74,7 +74,7 @@ def test_metadata_refuses(lib, bad, message):
 
 def logprob_args(**kw):
     a = dict(x=FAKE, dtype=1, T=8, V=1000, stride=1000, tokens=FAKE, temps=None, top=5, lp=FAKE, ent=FAKE, ids=FAKE, tlp=FAKE,
-             err=FAKE, stream=None)
+             ws=FAKE, wsb=1 << 30, err=FAKE, stream=None)
     assert set(kw) <= set(a)
     return list({**a, **kw}.values())
 
@@ -83,7 +83,7 @@ def logprob_args(**kw):
     (dict(dtype=7), b"dtype"), (dict(stride=999), b"sizes"), (dict(T=65536), b"sizes"), (dict(T=-1), b"sizes"),
     (dict(V=0), b"sizes"), (dict(V=(1 << 24) + 1, stride=1 << 25), b"sizes"), (dict(top=33), b"num_top"),
     (dict(top=-1), b"num_top"), (dict(V=4, top=5), b"num_top"), (dict(x=None), b"null"), (dict(ids=None), b"null"),
-    (dict(x=FAKE + 1), b"aligned")])
+    (dict(x=FAKE + 1), b"aligned"), (dict(ws=None), b"null"), (dict(ws=FAKE + 8), b"aligned")])
 def test_logprobs_refuse(lib, bad, message):
     assert lib.specdec_token_logprobs(*logprob_args(**bad)) == 1
     assert message in lib.specdec_last_error()

@@ -30,6 +30,7 @@ constexpr int kGroups = 64;          // groups of four threads
 constexpr int kMaxParts = 32;        // CTAs a row
 constexpr int kCandidates = 1024;    // holds every element of a part that fills fewer than kMaxTop groups
 constexpr int kErrToken = 8;
+constexpr int kSteps = 16, kMaxHits = 1024;      // a thread's steps are told apart modulo 16
 constexpr int kUnroll = 5;           // 16-byte vectors a thread has in flight
 
 // Ranks logits: larger first, the two zeros equal, NaN above all (but below the all-ones sentinel), ties to the lower index.
@@ -87,17 +88,24 @@ struct Row {
   __device__ __forceinline__ int whole_begin() const { return lead ? 1 : 0; }
   __device__ __forceinline__ int whole_end() const { return (lead + V) / kN; }
   __device__ __forceinline__ uint4 load(int v) const { return __ldg(base + v); }     // a whole vector
-  __device__ __noinline__ void edge(int v, float (&f)[kN]) const {                   // missing elements -inf
+  __device__ __noinline__ uint4 edge(int v) const {                                  // missing elements -inf
+    unsigned w[4] = {Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf};
+#pragma unroll
     for (int e = 0; e < kN; ++e) {
       const int i = index(v, e);
-      f[e] = i >= 0 && i < V ? to_f32(x[i]) : -INFINITY;
+      if (i < 0 || i >= V) continue;
+      if constexpr (kN == 4) {
+        w[e] = __float_as_uint(to_f32(x[i]));
+      } else {
+        const unsigned bits = reinterpret_cast<const unsigned short*>(x)[i];
+        w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | bits << 16 : (w[e / 2] & 0xffff0000u) | bits;
+      }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
   __device__ __forceinline__ void any(int v, float (&f)[kN]) const {
-    if (v >= whole_begin() && v < whole_end())
-      Vec<T>::unpack(load(v), f);
-    else
-      edge(v, f);
+    const uint4 raw = v >= whole_begin() && v < whole_end() ? load(v) : edge(v);
+    Vec<T>::unpack(raw, f);
   }
 };
 
@@ -109,7 +117,9 @@ struct Part {
 struct Shared {
   unsigned group[kGroups];
   unsigned bound;
-  int count, last;
+  int count, last, hits;
+  unsigned short step_high[kSteps][kThreads];    // upper half of the rank of a thread's largest in each of its steps
+  int hit[kMaxHits];                             // steps that reach the bound: step << 8 | thread
   unsigned long long list[kCandidates + 32], top[kMaxTop];
   float red_m[kThreads / 32], red_s[kThreads / 32], red_e[kThreads / 32];
   unsigned long long red_k[kThreads / 32];
@@ -150,12 +160,13 @@ __global__ void __launch_bounds__(kThreads, 5)
   const int v0 = min(r.nvec, part * per), v1 = min(r.nvec, v0 + per);
   const float temp = temps ? temps[row] : 1.0f;
   const float k2 = 1.4426950408889634f / temp;
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) sh.count = sh.hits = 0;
 
   // ---- one pass: running maximum, sum and weighted sum of this thread's elements (every kThreads-th vector of the part)
   float m = -FLT_MAX, s = 0.0f, e2 = 0.0f;
   const uint4 nothing = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
   const int w0 = max(v0, r.whole_begin()), w1 = min(v1, r.whole_end());
+  int step = 0;
   for (int v = v0 + tid; v < w1; v += kUnroll * kThreads) {
     uint4 raw[kUnroll];
 #pragma unroll
@@ -163,10 +174,16 @@ __global__ void __launch_bounds__(kThreads, 5)
       const int at = v + u * kThreads;
       raw[u] = at >= w0 && at < w1 ? r.load(at) : nothing;
     }
-    float mn = m;
+    float most = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) mn = fmaxf(mn, Vec<T>::most(raw[u]));
-    rebase(m, s, e2, mn, k2);
+    for (int u = 0; u < kUnroll; ++u) most = fmaxf(most, Vec<T>::most(raw[u]));
+    if (num_top > 0) {
+      const unsigned short h = (unsigned short)(rank_high(most) >> 16);
+      unsigned short& slot = sh.step_high[step % kSteps][tid];
+      slot = step < kSteps || h > slot ? h : slot;
+      ++step;
+    }
+    rebase(m, s, e2, fmaxf(m, most), k2);
     const float2 neg = make_float2(-m, -m), kk = make_float2(k2, k2);
     float2 ss = make_float2(0.0f, 0.0f), ee = ss;
 #pragma unroll
@@ -189,10 +206,11 @@ __global__ void __launch_bounds__(kThreads, 5)
     const int v = end ? r.whole_end() : 0;
     if ((end ? v >= r.nvec || v < r.whole_begin() : r.whole_begin() == 0) || v < v0 || v >= v1 || (v - v0) % kThreads != tid)
       continue;
-    float x[kN], mn = m;
-    r.edge(v, x);
-    for (int i = 0; i < kN; ++i) mn = fmaxf(mn, x[i]);
-    rebase(m, s, e2, mn, k2);
+    float x[kN];
+    const uint4 raw = r.edge(v);
+    Vec<T>::unpack(raw, x);
+    rebase(m, s, e2, fmaxf(m, Vec<T>::most(raw)), k2);
+#pragma unroll
     for (int i = 0; i < kN; ++i) {
       const float d = (x[i] - m) * k2, p = sm100::ex2_approx(d);
       s += p;
@@ -227,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, 5)
   bm = sh.red_m[0];
 #pragma unroll
   for (int w = 1; w < kThreads / 32; ++w) bm = fmaxf(bm, sh.red_m[w]);
+  const float s_own = s;
   rebase(m, s, e2, bm, k2);
   s = warp_sum_f32(s);
   e2 = warp_sum_f32(e2);
@@ -251,22 +270,41 @@ __global__ void __launch_bounds__(kThreads, 5)
   }
   if (num_top > 0) {
     const unsigned bound = sh.bound;
-    // the elements of each thread that reaches it, a vector a lane of its warp
-    for (unsigned hits = __ballot_sync(0xffffffffu, high >= bound); hits; hits &= hits - 1) {
-      const int first = v0 + warp * 32 + __ffs(hits) - 1;
-      for (int v = first + lane * kThreads; v < v1; v += 32 * kThreads) {
-        float x[kN];
-        r.any(v, x);
+    // the steps that reach it (all of a thread's that saw a NaN), then their vectors spread over the CTA, and the edges
+    const bool nan = s_own != s_own;
+    if (high >= bound)
+      for (int i = 0; i < min(step, kSteps); ++i)
+        if (nan || sh.step_high[i][tid] >= bound >> 16) {
+          const int at = atomicAdd(&sh.hits, 1);
+          if (at < kMaxHits) sh.hit[at] = i << 8 | tid;
+        }
+    __syncthreads();
+    auto consider = [&](int v) {
+      float x[kN];
+      r.any(v, x);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const int at = r.index(v, i);
-          if (rank_high(x[i]) >= bound && at >= 0 && at < V) {
-            const int slot = atomicAdd(&sh.count, 1);
-            if (slot < kCandidates) sh.list[slot] = rank_key(x[i], at);
-          }
+      for (int j = 0; j < kN; ++j) {
+        const int at = r.index(v, j);
+        if (rank_high(x[j]) >= bound && at >= 0 && at < V) {
+          const int slot = atomicAdd(&sh.count, 1);
+          if (slot < kCandidates) sh.list[slot] = rank_key(x[j], at);
         }
       }
+    };
+    constexpr int kStride = kUnroll * kThreads;
+    const int each = ((v1 - v0 + kStride - 1) / kStride + kSteps - 1) / kSteps * kUnroll;    // vectors a hit stands for
+    const int all = min(sh.hits, kMaxHits) * each;
+#pragma unroll 2
+    for (int i = tid; i < all; i += kThreads) {
+      const int hit = sh.hit[i / each], u = i % each;
+      const int v = v0 + (hit & 255) + ((hit >> 8) + u / kUnroll * kSteps) * kStride + u % kUnroll * kThreads;
+      if (v >= w0 && v < w1) consider(v);
     }
+    if (tid < 2) {
+      const int v = tid ? r.nvec - 1 : 0;
+      if (v >= v0 && v < v1 && (v < w0 || v >= w1) && (tid == 0 || v > 0)) consider(v);
+    }
+    if (tid == 0 && sh.hits > kMaxHits) atomicAdd(&sh.count, kCandidates + 1);       // not all looked at
     if (tid < num_top) sh.top[tid] = 0;
     __syncthreads();
     const int found = sh.count;
@@ -342,10 +380,10 @@ __global__ void __launch_bounds__(kThreads, 5)
   }
 }
 
-// CTAs a row: enough for six an SM over the rows, each thread left at least four vectors; one where the rows do that alone.
+// CTAs a row: enough for three an SM over the rows, each thread left at least four vectors; one where the rows do that alone.
 static int parts_of(long long rows, long long V, int dtype, int sm_count) {
   const long long vectors = V / (16 / (long long)dtype_bytes(dtype));
-  const long long wanted = (6LL * sm_count + rows - 1) / rows, most = vectors / (kThreads * 4);
+  const long long wanted = (3LL * sm_count + rows - 1) / rows, most = vectors / (kThreads * 4);
   const long long c = wanted < most ? wanted : most;
   return (int)(c < 1 ? 1 : c > kMaxParts ? kMaxParts : c);
 }

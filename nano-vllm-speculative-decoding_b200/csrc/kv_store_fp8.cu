@@ -14,11 +14,12 @@
 // x is stored as e4m3(x / scale), round to nearest even (half a step: 2^-4 of the value), infinities as +-448 * scale,
 // NaN as NaN.  A slot given twice holds its last token.
 //
-// One launch, no atomics on global memory, any order of slots: a token is its group's leader when no earlier token
-// of the call has a slot there; the leader's CTA scans the call's slots for the group's members (4 bytes a token,
-// from L1 / L2) and does the whole group, so each group and its scales are written by one CTA.  A CTA takes a run of
-// consecutive tokens, about one group's worth in a prompt.
+// One launch, no atomics on global memory, any order of slots: a token leads its group when no earlier token of the call
+// has a slot there; the leader's CTA looks over the call's slots (4 bytes a token, from L1 / L2) for the group's members and
+// does the whole group, so each group and its scales are written by one CTA.  A CTA takes some consecutive tokens, and one
+// of K and V (blockIdx.y); a warp takes a head's rows of a group into registers, 16 loads in flight.
 #include "common.cuh"
+#include "sm100.cuh"
 
 #include <cuda_fp8.h>
 
@@ -26,17 +27,20 @@ namespace specdec {
 namespace kv_fp8 {
 
 constexpr int kHeadDim = 128;
-constexpr int kThreads = 256;
+constexpr int kSideThreads = 256;       // of one side (K or V): a warp for each of 8 KV heads
+constexpr int kMaxChunk = 128;          // tokens of a CTA
 constexpr int kMinExponent = -100;
 constexpr int kMaxTokens = 16384;      // each leader scans the call's slots: bounds that scan
 
 struct StoreArgs {
-  const __nv_bfloat16* x[2];      // K rows, V rows [N][Hkv][128]
-  long long row_stride[2];
-  unsigned char* cache[2];        // [blocks][Hkv][block_size][128] e4m3
-  float* scale[2];                // [blocks][Hkv][block_size / group]
+  struct Side {
+    const __nv_bfloat16* x;       // rows [N][Hkv][128]
+    long long row_stride;
+    unsigned char* cache;         // [blocks][Hkv][block_size][128] e4m3
+    float* scale;                 // [blocks][Hkv][block_size / group]
+  } k, v;
   const int* slots;               // [N]
-  int N, chunk, Hkv, block_size;
+  int N, N4, chunk, Hkv, block_size;   // N4: whole 16-byte quads of slots (0: the mapping is not 16-byte aligned)
   long long num_slots;
   int* err;
 };
@@ -66,75 +70,183 @@ __device__ __forceinline__ float2 decode2(unsigned pair) {
   return __half22float2(__half2(h));
 }
 
-template <int GROUP>
-__global__ void __launch_bounds__(kThreads) store_fp8_kernel(const StoreArgs a) {
-  __shared__ int winner[GROUP];    // the group's members: the last token of each slot, or -1
-  __shared__ int earlier;          // a token before this one has a slot of the group
+// kWide: K and V in one CTA of two sides' threads, many tokens a CTA; else blockIdx.y is the side.
+template <int GROUP, bool kWide>
+__global__ void __launch_bounds__(kWide ? 2 * kSideThreads : kSideThreads, kWide ? 1 : GROUP == 16 ? 4 : 2)
+    store_fp8_kernel(const StoreArgs a) {
+  constexpr int kThreads = kWide ? 2 * kSideThreads : kSideThreads;
+  // The chunk's groups: the first slot of each, the token that leads it, its members (the last token of each slot, or -1)
+  // and whether an earlier token of the call has a slot of it (another CTA's then, or an earlier entry's).
+  __shared__ int first_slot[kMaxChunk], leader[kMaxChunk], winner[kMaxChunk][GROUP];
+  __shared__ unsigned char earlier[kMaxChunk];
+  __shared__ unsigned filter[32];
+  __shared__ int count;
   griddep_launch_dependents();
   griddep_wait();                  // may be launched as a dependent of the kernel that wrote its input
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const StoreArgs::Side side = (kWide ? warp >= kSideThreads / 32 : blockIdx.y) ? a.v : a.k;
   const int t_begin = blockIdx.x * a.chunk, t_end = min(a.N, t_begin + a.chunk);
-  for (int t = t_begin; t < t_end; ++t) {             // uniform over the CTA
-    const int slot = a.slots[t];
+  if (threadIdx.x == 0) count = 0;
+  if (threadIdx.x < 32) filter[threadIdx.x] = 0;
+  __syncthreads();
+  for (int t = t_begin + threadIdx.x; t < t_end; t += kThreads) {
+    const int slot = a.slots[t], before = t > 0 ? a.slots[t - 1] : -1;
     if (slot < 0) continue;
     if (slot >= a.num_slots) {
-      if (threadIdx.x == 0) atomicCAS(a.err, 0, 3);
+      atomicCAS(a.err, 0, 3);
       continue;
     }
-    const int g0 = slot / GROUP * GROUP;              // the group's first slot
-    if (t > 0 && (unsigned)(a.slots[t - 1] - g0) < (unsigned)GROUP) continue;
-    __syncthreads();
-    if (threadIdx.x < GROUP) winner[threadIdx.x] = -1;
-    if (threadIdx.x == 0) earlier = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < a.N; i += kThreads) {
-      const unsigned o = (unsigned)(a.slots[i] - g0);
+    const int g0 = slot / GROUP * GROUP;
+    if ((unsigned)(before - g0) < (unsigned)GROUP) continue;       // not a run's first token
+    const int l = atomicAdd(&count, 1);
+    first_slot[l] = g0;
+    leader[l] = t;
+    earlier[l] = 0;
+  }
+  __syncthreads();
+  const int groups = count;
+  if (groups == 0) return;
+  for (int i = threadIdx.x; i < groups * GROUP; i += kThreads) winner[i / GROUP][i % GROUP] = -1;
+  // every slot of the call against the chunk's groups; a bit for each group number modulo 1024 turns nearly all others away
+  for (int l = threadIdx.x; l < groups; l += kThreads) {
+    const unsigned g = (unsigned)first_slot[l] / GROUP;
+    atomicOr(&filter[g / 32 % 32], 1u << (g % 32));
+  }
+  __syncthreads();
+  auto member = [&](int slot, int i) {
+    const unsigned g = (unsigned)slot / GROUP;
+    if (!(filter[g / 32 % 32] >> (g % 32) & 1)) return;
+    for (int l = 0; l < groups; ++l) {
+      const unsigned o = (unsigned)(slot - first_slot[l]);
       if (o < (unsigned)GROUP) {
-        atomicMax(&winner[o], i);
-        if (i < t) earlier = 1;
+        atomicMax(&winner[l][o], i);
+        if (i < leader[l]) earlier[l] = 1;
       }
     }
-    __syncthreads();
-    if (earlier) continue;
-    const bool started = winner[0] >= 0;
-    const int block = g0 / a.block_size, j0 = g0 % a.block_size;
-    for (int u = warp; u < 2 * a.Hkv; u += kThreads / 32) {
-      const int side = u >= a.Hkv, h = u - side * a.Hkv;
-      const __nv_bfloat16* x = a.x[side] + h * kHeadDim + lane * 4;
-      uint2 v[GROUP];
-      unsigned most = 0;
+  };
+  constexpr int kAhead = 4;
+  for (int i0 = threadIdx.x; i0 < a.N4; i0 += kAhead * kThreads) {
+    int4 four[kAhead];
 #pragma unroll
-      for (int o = 0; o < GROUP; ++o) {
-        const int w = winner[o];
-        v[o] = w >= 0 ? *reinterpret_cast<const uint2*>(x + w * a.row_stride[side]) : make_uint2(0u, 0u);
-      }
+    for (int u = 0; u < kAhead; ++u) four[u] = __ldg(reinterpret_cast<const int4*>(a.slots) + min(i0 + u * kThreads, a.N4 - 1));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i >= a.N4) break;
+      member(four[u].x, 4 * i);
+      member(four[u].y, 4 * i + 1);
+      member(four[u].z, 4 * i + 2);
+      member(four[u].w, 4 * i + 3);
+    }
+  }
+  for (int i = 4 * a.N4 + threadIdx.x; i < a.N; i += kThreads) member(a.slots[i], i);
+  __syncthreads();
+  // A warp's units: its heads of each group.  fetch issues a unit's loads, finish turns them into codes.
+  constexpr int kHeadWarps = kSideThreads / 32;
+  const int h0 = warp % kHeadWarps;
+  auto first_group = [&](int l) {
+    while (l < groups && earlier[l]) ++l;
+    return l;
+  };
+  auto fetch = [&](int l, int h, uint2 (&v)[GROUP], float& old) {
+    const int mine = lane < GROUP ? winner[l][lane] : -1;
+    const int source = mine >= 0 ? mine : leader[l];      // the row read for a slot that the call does not write: any of its own
+    const int g0 = first_slot[l];
+    old = side.scale[((long long)(g0 / a.block_size) * a.Hkv + h) * (a.block_size / GROUP) + g0 % a.block_size / GROUP];
+    const __nv_bfloat16* x = side.x + h * kHeadDim + lane * 4;
+#pragma unroll
+    for (int o = 0; o < GROUP; ++o)          // unconditional, so that all are in flight at once: a branch would serialise them
+      v[o] = *reinterpret_cast<const uint2*>(x + __shfl_sync(0xffffffffu, source, o) * side.row_stride);
+  };
+  auto finish = [&](int l, int h, uint2 (&v)[GROUP], float old) {
+    const unsigned members = __ballot_sync(0xffffffffu, lane < GROUP && winner[l][lane % GROUP] >= 0);
+    const bool started = members & 1;
+    const int g0 = first_slot[l], j0 = g0 % a.block_size;
+    const long long head = (long long)(g0 / a.block_size) * a.Hkv + h;
+    constexpr unsigned kAllSlots = GROUP == 32 ? 0xffffffffu : (1u << (GROUP % 32)) - 1u;
+    if (members != kAllSlots) {
+#pragma unroll
+      for (int o = 0; o < GROUP; ++o)
+        if (!(members >> o & 1)) v[o] = make_uint2(0u, 0u);
+    }
+    // the largest magnitude, in packed pairs (the maximum drops NaN); an infinity has it taken again without them
+    __nv_bfloat162 most2 = as_h2<__nv_bfloat162>(0u);
+#pragma unroll
+    for (int o = 0; o < GROUP; ++o)
+      most2 = __hmax2(most2, __hmax2(as_h2<__nv_bfloat162>(v[o].x & 0x7fff7fffu), as_h2<__nv_bfloat162>(v[o].y & 0x7fff7fffu)));
+    unsigned most = max(__bfloat16_as_ushort(__low2bfloat16(most2)), __bfloat16_as_ushort(__high2bfloat16(most2)));
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (most >= 0x7f80u) {
+      most = 0;
 #pragma unroll
       for (int o = 0; o < GROUP; ++o) most = max(most, max(finite_magnitude(v[o].x), finite_magnitude(v[o].y)));
       most = __reduce_max_sync(0xffffffffu, most);
-      const long long head = (long long)block * a.Hkv + h;
-      float* scale = a.scale[side] + head * (a.block_size / GROUP) + j0 / GROUP;
-      const float old = *scale, wanted = scale_for(most);
-      const float now = started ? wanted : fmaxf(old, wanted);
-      const float inv = 1.0f / now;
-      const bool rescale = !started && now > old;
-      const float ratio = old * inv;
-      unsigned* row = reinterpret_cast<unsigned*>(a.cache[side] + (head * a.block_size + j0) * kHeadDim) + lane;
+    }
+    const float wanted = scale_for(most);
+    const float now = started ? wanted : fmaxf(old, wanted);
+    const float inv = 1.0f / now;
+    const bool rescale = !started && now > old;
+    const float ratio = old * inv;
+    unsigned* row = reinterpret_cast<unsigned*>(side.cache + (head * a.block_size + j0) * kHeadDim) + lane;
+    const float2 k2 = make_float2(inv, inv);
+    auto code = [&](uint2 r) {
+      const float2 lo = sm100::mul_x2(make_float2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u)), k2);
+      const float2 hi = sm100::mul_x2(make_float2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)), k2);
+      return encode4(lo.x, lo.y, hi.x, hi.y);
+    };
+    if (members == kAllSlots) {                 // a whole group: straight through
+#pragma unroll
+      for (int o = 0; o < GROUP; ++o) row[o * (kHeadDim / 4)] = code(v[o]);
+    } else {
 #pragma unroll
       for (int o = 0; o < GROUP; ++o) {
         unsigned* p = row + o * (kHeadDim / 4);
-        if (winner[o] >= 0) {
-          *p = encode4(__uint_as_float(v[o].x << 16) * inv, __uint_as_float(v[o].x & 0xffff0000u) * inv,
-                       __uint_as_float(v[o].y << 16) * inv, __uint_as_float(v[o].y & 0xffff0000u) * inv);
+        if (members >> o & 1) {
+          *p = code(v[o]);
         } else if (rescale) {
           const unsigned c = *p;
           const float2 lo = decode2(c), hi = decode2(c >> 16);
           *p = encode4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
         }
       }
-      __syncwarp();
-      if (lane == 0 && now != old) *scale = now;
     }
+    __syncwarp();
+    if (lane == 0 && now != old) side.scale[head * (a.block_size / GROUP) + j0 / GROUP] = now;
+  };
+  uint2 v[GROUP];
+  float old;
+  if constexpr (kWide && GROUP == 16) {       // the next unit's loads pass under this one's arithmetic
+    uint2 v2[GROUP];
+    float old2;
+    auto next = [&](int& l, int& h) {
+      h += kHeadWarps;
+      if (h >= a.Hkv) {
+        h = h0;
+        l = first_group(l + 1);
+      }
+    };
+    int l = first_group(0), h = h0;
+    if (h0 >= a.Hkv || l >= groups) return;
+    fetch(l, h, v, old);
+    for (;;) {
+      int l2 = l, h2 = h;
+      next(l2, h2);
+      if (l2 < groups) fetch(l2, h2, v2, old2);
+      finish(l, h, v, old);
+      if (l2 >= groups) break;
+      l = l2;
+      h = h2;
+      next(l, h);
+      if (l < groups) fetch(l, h, v, old);
+      finish(l2, h2, v2, old2);
+      if (l >= groups) break;
+    }
+  } else {
+    for (int l = first_group(0); l < groups; l = first_group(l + 1))
+      for (int h = h0; h < a.Hkv; h += kHeadWarps) {
+        fetch(l, h, v, old);
+        finish(l, h, v, old);
+      }
   }
 }
 
@@ -168,28 +280,30 @@ int specdec_store_kvcache_fp8(const void* key, long long key_row_stride, const v
   DeviceInfo info;
   if (int st = device_info(&info)) return st;
   StoreArgs a{};
-  a.x[0] = static_cast<const __nv_bfloat16*>(key);
-  a.x[1] = static_cast<const __nv_bfloat16*>(value);
-  a.row_stride[0] = key_row_stride;
-  a.row_stride[1] = value_row_stride;
-  a.cache[0] = static_cast<unsigned char*>(k_cache);
-  a.cache[1] = static_cast<unsigned char*>(v_cache);
-  a.scale[0] = k_scale;
-  a.scale[1] = v_scale;
+  a.k = {static_cast<const __nv_bfloat16*>(key), key_row_stride, static_cast<unsigned char*>(k_cache), k_scale};
+  a.v = {static_cast<const __nv_bfloat16*>(value), value_row_stride, static_cast<unsigned char*>(v_cache), v_scale};
   a.slots = slot_mapping;
   a.N = (int)N;
+  a.N4 = (reinterpret_cast<uintptr_t>(slot_mapping) & 15) == 0 ? (int)(N / 4) : 0;
   a.Hkv = num_kv_heads;
   a.block_size = block_size;
   a.num_slots = num_blocks * block_size;
   a.err = err;
-  const int most = 8 * info.sm_count;
-  a.chunk = (int)((N + most - 1) / most);
-  const dim3 grid((unsigned)((N + a.chunk - 1) / a.chunk));
+  // Tokens a CTA: one while the GPU holds that many CTAs at once (each token of a decode is a group of its own).  More of
+  // them come from a prompt: a CTA an SM, which looks over the call's slots once for all its groups (the looks' total grows
+  // with the CTAs) and loads one group's rows while it converts another's.
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (scale_group == 16)
-    SPECDEC_CUDA_TRY(launch_dependent(store_fp8_kernel<16>, grid, dim3(kThreads), s, a));
+  const bool wide = N > 8 * info.sm_count;
+  a.chunk = wide ? (int)((N + info.sm_count - 1) / info.sm_count) : 1;
+  if (a.chunk > kMaxChunk) a.chunk = kMaxChunk;
+  const unsigned ctas = (unsigned)((N + a.chunk - 1) / a.chunk);
+  const dim3 grid(ctas, wide ? 1 : 2), block(wide ? 2 * kSideThreads : kSideThreads);
+  if (wide)
+    SPECDEC_CUDA_TRY(scale_group == 16 ? launch_dependent(store_fp8_kernel<16, true>, grid, block, s, a)
+                                       : launch_dependent(store_fp8_kernel<32, true>, grid, block, s, a));
   else
-    SPECDEC_CUDA_TRY(launch_dependent(store_fp8_kernel<32>, grid, dim3(kThreads), s, a));
+    SPECDEC_CUDA_TRY(scale_group == 16 ? launch_dependent(store_fp8_kernel<16, false>, grid, block, s, a)
+                                       : launch_dependent(store_fp8_kernel<32, false>, grid, block, s, a));
   SPECDEC_LAUNCH_CHECK();
   return kOk;
 }

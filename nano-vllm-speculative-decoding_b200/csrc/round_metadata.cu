@@ -56,7 +56,7 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
           length + n - 1 > (long long)a.table_width * a.block_size;
   x.n = x.bad ? 0 : (int)n;
   if (x.bad) x.start = 0;
-  x.need = (int)((x.start + x.n + a.block_size - 1) / a.block_size);
+  x.need = (int)(((unsigned)(x.start + x.n) + (unsigned)a.block_size - 1u) / (unsigned)a.block_size);   // below 2^31 here
   if (!x.bad && (max(x.need, x.held) > a.width || (!a.free_blocks && x.need > x.held))) x.bad = 1;
   return x;
 }
@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
   // sums over the rows before r and over all rows: tokens, keys, new blocks
   int tokens = 0, all_tokens = 0, fresh = 0, all_fresh = 0, bad = 0;
   long long keys = 0, all_keys = 0;
+#pragma unroll 4
   for (int i = lane; i < a.R; i += 32) {
     const Row x = row_of(a, i);
     const int f = max(0, x.need - x.held);
@@ -147,12 +148,12 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
     }
     __syncwarp();
     for (int j = lane; j < n; j += 32) {
-      const long long pos = start + j;
+      const unsigned pos = (unsigned)start + j, bs = (unsigned)a.block_size;
       const int t = first + j;
       const bool real = r < a.R;
       a.positions[t] = pos;
       a.input_ids[t] = !real ? 0 : j == 0 ? a.last_tokens[r] : a.drafts ? a.drafts[(long long)r * a.k + j - 1] : 0;
-      a.slots[t] = real ? table[pos / a.block_size] * a.block_size + (int)(pos % a.block_size) : -1;
+      a.slots[t] = real ? table[pos / bs] * a.block_size + (int)(pos % bs) : -1;
     }
   }
   if (idle)                           // no row has tokens: the whole token range is padding

@@ -10,6 +10,8 @@ no host round trip.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib
@@ -17,9 +19,32 @@ from ._lib import Workspace, call_on, ptr, raw_stream, require_cuda, same_device
 from .batch_metadata import packed_sizes
 
 
+@dataclass
+class DeviceRows:
+    """The requests of a batch on the GPU: what verify_metadata reads of them, and the free blocks they grow into."""
+    lengths: torch.Tensor        # [R] int64: tokens of each row, the last one included
+    last_tokens: torch.Tensor    # [R] int64
+    block_tables: torch.Tensor   # [R, W] int32
+    num_blocks: torch.Tensor     # [R] int32: blocks each row holds
+    free_blocks: torch.Tensor | None = None   # [capacity] int32 stack
+    free_count: torch.Tensor | None = None    # [1] int32
+
+    def advance(self, n_accept: torch.Tensor, tail: torch.Tensor, error: torch.Tensor) -> None:
+        """A round's outcome: every row is longer by its accepted drafts and the tail token, which is its last now.
+        Nothing changes where error, an int32 word on the device, is set."""
+        done = error == 0
+        self.lengths.add_((n_accept + 1) * done)
+        self.last_tokens.copy_(torch.where(done, tail, self.last_tokens))
+
+
 def _words(device: torch.device) -> torch.Tensor:
     """[error word, ticket] of this device."""
     return Workspace.get(device, 256, name="device_metadata")[:8].view(torch.int32)
+
+
+def error_word(device: torch.device) -> torch.Tensor:
+    """The int32 word that device_error reads, on the device."""
+    return _words(device)[0]
 
 
 def device_error(device: torch.device) -> int:

@@ -4,6 +4,7 @@
     silu_and_mul(gate_up)                   nanovllm/layers/activation.py:8-11  -> specdec_silu_mul
     qk_norm_rope_store(...)                 nanovllm/models/qwen3.py:77-86 + attention.py:62-63
                                             (q_norm, k_norm, RoPE, store_kvcache in one launch) -> specdec_norm_rope_store
+    qk_norm_rope(...)                       the same without the cache: q, k, v rows in token order
     rope_cache(head_dim, max_position, base) nanovllm/layers/rotary_embedding.py:17-27 (the cos|sin table)
 """
 from __future__ import annotations
@@ -68,3 +69,13 @@ def qk_norm_rope_store(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, q_n
         cos_sin.shape[0], ptr(positions), ptr(slot_mapping), ptr(k_cache), ptr(v_cache), 0, num_slots, ptr(q_out),
         float(eps), ptr(err_word(device)), stream_of(device)))
     return q_out
+
+
+def qk_norm_rope(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                 cos_sin: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, eps: float
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """qk_norm_rope_store with the K and V rows kept in token order instead of a cache's slots (for a store of another
+    format): q [T, H, 128], k and v [T, Hkv, 128].  rows: int32 0 .. T-1 on the device."""
+    k, v = (torch.empty(qkv.shape[0], num_kv_heads, 128, dtype=qkv.dtype, device=qkv.device) for _ in range(2))
+    q = qk_norm_rope_store(qkv, num_heads, num_kv_heads, q_norm, k_norm, cos_sin, positions, rows, k, v, eps)
+    return q, k, v

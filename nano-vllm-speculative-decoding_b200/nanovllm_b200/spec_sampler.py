@@ -62,6 +62,12 @@ def sampling_tensors(seqs, device: torch.device) -> SamplingTensors:
     )
 
 
+def status_word(device: torch.device) -> torch.Tensor:
+    """The int32 word on the device that tells whether the last acceptance refused its inputs (0: it did not; its
+    outputs are undefined otherwise): lengths out of range or not summing to the logits' rows, draft ids, top_k."""
+    return Workspace.get(device, 256)[:4].view(torch.int32)[0]
+
+
 def sampling_per_token(sampling: SamplingTensors, verified_lens: torch.Tensor, num_tokens: int) -> SamplingTensors:
     """spec_sampler.py:44-52: each row's parameters repeated over its verified positions."""
     temperatures = sampling.temperatures

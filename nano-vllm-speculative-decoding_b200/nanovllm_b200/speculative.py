@@ -26,6 +26,8 @@ import torch
 from . import spec_sampler
 from .batch_metadata import (RowState, draft_packed_sizes, draft_packed_views, draft_placement,
                              pack_draft_block_metadata, pack_verify_metadata)
+from .device_metadata import DeviceRows, error_word, verify_metadata
+from .logprobs import TokenLogprobs, token_logprobs
 from .markov import MarkovQBuffer, markov_rows, num_candidates
 from .spec_sampler import SamplingTensors
 from .target import Qwen3Target
@@ -65,6 +67,7 @@ class VerifyRound:
         self.pinned: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
         self.placement: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}   # pinned host | device, per graph
         self.loaded: dict[int, tuple[int, int, int]] = {}   # per graph: verified tokens, rows, drafts placed
+        self.device_lens: dict[int, torch.Tensor | None] = {}   # per graph loaded by load_device: its verified lengths
         query_len = num_drafts + 1
         self.shapes: dict[int, int] = {}
         for rows in graph_rows:
@@ -123,6 +126,7 @@ class VerifyRound:
         num_verified = sum(lens)
         num_tokens = self.graph_for(len(rows), num_verified)
         self._load(self.target.graphs[num_tokens][1], rows, lens, self.shapes[num_tokens], num_tokens)
+        self.device_lens.pop(num_tokens, None)
         placed = -1                                            # fixed-length: rows are contiguous k + 1 blocks
         if verified_lens is not None:
             index, source = draft_placement(lens, k)
@@ -136,6 +140,28 @@ class VerifyRound:
         self.loaded[num_tokens] = (num_verified, len(rows), placed)
         return num_tokens
 
+    def load_device(self, rows: DeviceRows, drafts: torch.Tensor, verified_lens: torch.Tensor | None = None,
+                    num_verified: int | None = None) -> int:
+        """load for requests kept on the GPU: the metadata, the drafts among the input ids and the blocks that the rows
+        lack, in one launch and no host copy (device_metadata.verify_metadata).  verified_lens [R] int64 on the device
+        needs their sum, num_verified, on the host.  Returns the graph's token count."""
+        n, k = drafts.shape
+        if k != self.num_drafts:
+            raise ValueError(f"{k} drafts a row, {self.num_drafts} expected")
+        if verified_lens is None:
+            num_verified = n * (k + 1)
+        elif num_verified is None:
+            raise ValueError("verified_lens needs num_verified, their sum")
+        num_tokens = self.graph_for(n, num_verified)
+        b = self.target.graphs[num_tokens][1]
+        verify_metadata(rows.lengths, rows.last_tokens, drafts, verified_lens, rows.block_tables, rows.num_blocks,
+                        rows.free_blocks, rows.free_count, block_size=self.block_size, num_rows=self.shapes[num_tokens],
+                        num_tokens=num_tokens, pad_block_id=self.target.pad_block_id, width=self.max_num_blocks,
+                        buf64=b["_packed64"], buf32=b["_packed32"])
+        self.loaded[num_tokens] = (num_verified, n, -1)
+        self.device_lens[num_tokens] = verified_lens
+        return num_tokens
+
     def place_drafts(self, num_tokens: int, drafts: torch.Tensor) -> torch.Tensor | None:
         """speculative.py:514-517: the verified drafts into the graph's input ids where the loaded metadata puts
         them.  Returns the device verified lengths of a variable-length round (None for fixed-length rows)."""
@@ -144,6 +170,8 @@ class VerifyRound:
         batch, k = drafts.shape
         if batch != n:
             raise ValueError(f"drafts for {batch} rows, metadata loaded for {n}")
+        if num_tokens in self.device_lens:                     # load_device has placed them
+            return self.device_lens[num_tokens]
         if placed < 0:
             buffers["input_ids"][:batch * (k + 1)].view(batch, k + 1)[:, 1:].copy_(drafts)
             return None
@@ -169,6 +197,44 @@ class VerifyRound:
     def logits(self, num_tokens: int) -> torch.Tensor:
         """The last replay's logits of the verified tokens, [T, V] bf16 (valid until the next replay)."""
         return self.target.graphs[num_tokens][1]["logits"][:self.loaded[num_tokens][0]]
+
+    def emitted_logprobs(self, num_tokens: int, drafts: torch.Tensor, n_accept: torch.Tensor, tail: torch.Tensor,
+                         num_top: int = 0, verified_lens: torch.Tensor | None = None) -> TokenLogprobs:
+        """The last replay's log probabilities of the tokens that the round emitted: position j of a row's verified
+        tokens holds its emitted token j (accepted drafts, then the tail); later positions emitted none (0, ids -1)."""
+        num_verified, n, _ = self.loaded[num_tokens]
+        k = drafts.shape[1]
+        device = drafts.device
+        every = torch.cat([drafts, tail.unsqueeze(1)], dim=1)
+        j = torch.arange(k + 1, device=device)
+        emitted = torch.where(j == n_accept.unsqueeze(1), tail.unsqueeze(1), every)
+        emitted = torch.where(j <= n_accept.unsqueeze(1), emitted, -1)
+        if verified_lens is None:
+            tokens = emitted.reshape(-1)
+        else:
+            # by search and clamps, not repeat_interleave: lengths of another sum must not index past the tensors
+            ends = verified_lens.cumsum(0)
+            flat = torch.arange(num_verified, device=device)
+            row = torch.searchsorted(ends, flat, right=True).clamp_(max=n - 1)
+            place = flat - (ends - verified_lens)[row]
+            tokens = torch.where(place <= k, emitted[row, place.clamp(0, k)], -1)
+        return token_logprobs(self.logits(num_tokens), tokens, num_top)
+
+    def run_round_device(self, rows: DeviceRows, drafts: torch.Tensor, draft_probs: torch.Tensor | None,
+                         sampling: SamplingTensors, generator: torch.Generator | None = None,
+                         verified_lens: torch.Tensor | None = None, num_verified: int | None = None,
+                         num_top: int | None = None) -> tuple[torch.Tensor, torch.Tensor, TokenLogprobs | None]:
+        """run_round with the requests on the GPU and no host copy in either direction: returns n_accept [R], tail [R]
+        and, with num_top, the emitted tokens' log probabilities (emitted_logprobs); rows are advanced.  Where the
+        metadata recorded an error (device_metadata.device_error: the free blocks ran out, lengths out of range) the round
+        has stored nothing, its results are void and the rows stay as they were, until the error is reset; where the
+        acceptance refused its inputs, lengths of another sum than num_verified say, they stay for this round."""
+        num_tokens = self.load_device(rows, drafts, verified_lens, num_verified)
+        n_accept, tail = self.verify_and_accept(num_tokens, drafts.shape[0], drafts, draft_probs, sampling, generator)
+        logprobs = (None if num_top is None else
+                    self.emitted_logprobs(num_tokens, drafts, n_accept, tail, num_top, verified_lens))
+        rows.advance(n_accept, tail, error_word(drafts.device) | spec_sampler.status_word(drafts.device))
+        return n_accept, tail, logprobs
 
     def commit(self, drafts: torch.Tensor, n_accept: torch.Tensor, tail: torch.Tensor,
                verified_lens: list[int] | None) -> list[list[int]]:

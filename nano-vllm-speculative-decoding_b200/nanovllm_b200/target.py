@@ -10,7 +10,8 @@ The projections and the LM head are plain cuBLAS GEMMs (torch.matmul); everythin
 package's kernels: RMSNorm(+residual), q/k norm + RoPE + paged K/V store, paged verify attention (kernel 2) and
 SiLU*mul.  Weights are random-initialised (no checkpoints here); the paged KV cache is [2, layers, blocks + 1,
 block_size, Hkv, 128] with the last block the zeroed pad block, as ModelRunner.allocate_kv_cache lays it out
-(nanovllm/engine/model_runner.py:142-169).  A whole verification (forward + logits) is captured as one CUDA
+(nanovllm/engine/model_runner.py:142-169); with kv_dtype float8_e4m3fn it is an 8-bit cache a layer
+(nanovllm_b200.attention_fp8), its pad block zero too.  A whole verification (forward + logits) is captured as one CUDA
 graph per token count, replayed with the round's metadata copied into its static buffers.
 """
 from __future__ import annotations
@@ -20,6 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import attention, fused
+from .attention_fp8 import FP8Cache, paged_attention_fp8, store_kvcache_fp8
 
 
 @dataclass
@@ -49,19 +51,23 @@ def random_layer_weights(s: Qwen3Shape, rand, norm_weight) -> dict:
 
 def decoder_layer(s: Qwen3Shape, w: dict, layer_id: int, h: torch.Tensor, residual: torch.Tensor | None,
                   positions: torch.Tensor, slot_mapping: torch.Tensor, kv_cache: torch.Tensor,
-                  cos_sin: torch.Tensor, attend) -> tuple[torch.Tensor, torch.Tensor]:
+                  cos_sin: torch.Tensor, attend, store=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Qwen3DecoderLayer.forward (qwen3.py:147-160) on this package's kernels: input RMSNorm (+residual), the
     qkv GEMM, q/k norm + RoPE with the K/V rows stored at slot_mapping into layer `layer_id` of kv_cache, then
     attend(q, layer_id) (the paged branch the caller picks: varlen verify or the draft block), o_proj, the
-    post-attention RMSNorm and the SiLU-gated MLP.  Returns (hidden, residual) like the reference's layer."""
+    post-attention RMSNorm and the SiLU-gated MLP.  Returns (hidden, residual) like the reference's layer.  store,
+    when given, takes the place of the norm, RoPE and bf16 store: store(qkv, w, layer_id) -> q (kv_cache is not used)."""
     T = h.shape[0]
     if residual is None:
         x, residual = fused.rmsnorm(h, w["in_norm"], s.eps), h
     else:
         x, residual = fused.rmsnorm(h, w["in_norm"], s.eps, residual=residual)
     qkv = torch.matmul(x, w["w_qkv"].t())
-    q = fused.qk_norm_rope_store(qkv, s.heads, s.kv_heads, w["q_norm"], w["k_norm"], cos_sin, positions,
-                                 slot_mapping, kv_cache[0, layer_id], kv_cache[1, layer_id], s.eps)
+    if store is not None:
+        q = store(qkv, w, layer_id)
+    else:
+        q = fused.qk_norm_rope_store(qkv, s.heads, s.kv_heads, w["q_norm"], w["k_norm"], cos_sin, positions,
+                                     slot_mapping, kv_cache[0, layer_id], kv_cache[1, layer_id], s.eps)
     o = attend(q, layer_id)
     h = torch.matmul(o.view(T, -1), w["w_o"].t())
     x, residual = fused.rmsnorm(h, w["post_norm"], s.eps, residual=residual)
@@ -71,7 +77,7 @@ def decoder_layer(s: Qwen3Shape, w: dict, layer_id: int, h: torch.Tensor, residu
 
 class Qwen3Target:
     def __init__(self, shape: Qwen3Shape, device: torch.device, num_blocks: int, block_size: int = 256,
-                 seed: int = 0, init_scale: float = 0.02):
+                 seed: int = 0, init_scale: float = 0.02, kv_dtype: torch.dtype = torch.bfloat16):
         self.shape = s = shape
         self.device = device
         self.block_size = block_size
@@ -90,8 +96,14 @@ class Qwen3Target:
         self.layers = [random_layer_weights(s, rand, norm_weight) for _ in range(s.layers)]
         self.final_norm = norm_weight(s.hidden)
         self.lm_head = rand(s.vocab, s.hidden)
-        self.kv_cache = torch.zeros(2, s.layers, num_blocks + 1, block_size, s.kv_heads, s.head_dim, dtype=bf,
-                                    device=device)
+        self.kv_cache = self.kv_fp8 = None
+        if kv_dtype == torch.float8_e4m3fn:     # one attention_fp8.FP8Cache a layer, half the bytes of the bf16 cache
+            self.kv_fp8 = [FP8Cache.allocate(num_blocks + 1, block_size, s.kv_heads, device) for _ in range(s.layers)]
+        elif kv_dtype == bf:
+            self.kv_cache = torch.zeros(2, s.layers, num_blocks + 1, block_size, s.kv_heads, s.head_dim, dtype=bf,
+                                        device=device)
+        else:
+            raise ValueError(f"kv_dtype {kv_dtype}: bfloat16 or float8_e4m3fn")
         self.cos_sin = fused.rope_cache(s.head_dim, s.max_position, s.rope_theta, device)
         self.scale = s.head_dim ** -0.5
         # error words / workspaces exist before any graph capture
@@ -107,7 +119,23 @@ class Qwen3Target:
         aux layers' outputs (hidden + residual, qwen3.py:186-190)."""
         s = self.shape
 
+        store = None
+        if self.kv_fp8 is not None:
+            rows = torch.arange(input_ids.shape[0], dtype=torch.int32, device=self.device)
+
+            def store(qkv, w, layer_id):
+                c = self.kv_fp8[layer_id]
+                q, k, v = fused.qk_norm_rope(qkv, s.heads, s.kv_heads, w["q_norm"], w["k_norm"], self.cos_sin, positions,
+                                             rows, s.eps)
+                store_kvcache_fp8(k, v, c.k_cache, c.v_cache, c.k_scale, c.v_scale, slot_mapping)
+                return q
+
         def attend(q, layer_id):
+            if self.kv_fp8 is not None:
+                c = self.kv_fp8[layer_id]
+                return paged_attention_fp8(q, c.k_cache, c.v_cache, c.k_scale, c.v_scale, block_tables, self.scale,
+                                           cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
+                                           max_seqlen_q=max_seqlen_q, early_launch=True)
             # launched early: its predecessor (the q/k norm, RoPE and K/V store) writes q and the caches only
             return attention.paged_attention(q, self.kv_cache[0, layer_id], self.kv_cache[1, layer_id], block_tables,
                                              self.scale, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
@@ -117,7 +145,7 @@ class Qwen3Target:
         residual = None
         for layer_id, w in enumerate(self.layers):
             h, residual = decoder_layer(s, w, layer_id, h, residual, positions, slot_mapping, self.kv_cache,
-                                        self.cos_sin, attend)
+                                        self.cos_sin, attend, store)
             if aux_out is not None and layer_id in s.aux_layer_ids:
                 seg = s.aux_layer_ids.index(layer_id)
                 aux_out[:, seg * s.hidden:(seg + 1) * s.hidden].copy_(h + residual)

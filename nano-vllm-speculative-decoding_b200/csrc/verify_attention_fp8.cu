@@ -35,6 +35,13 @@
 // independent tiles' arithmetic to interleave (16k contexts: 379 -> 362 us; one tile ahead in software instead: 595 us).
 // The MMA warp runs converged with a predicated leader lane: issued from a divergent lane an MMA cost about 100 clocks,
 // more than its execution (429 -> 376 us).  Rings deeper than this lost time (5 stages of K and V: 15 % at 3k contexts).
+// Measured (32 query and 8 KV heads): 64 rows of 1 to 8 queries on 16k contexts 347 to 367 us (2144 MB, 0.90 to 0.95 of the
+// copy rate; the bf16 kernel on its cache 630 to 674 us) where the SMs hold 1.9 GHz; called for seconds on end the GPU
+// reaches its 1000 W and the clock falls to 1.5 to 1.7 GHz: 390 to 430 us, a pair's 2700 clocks being the softmax's chain
+// then.  64 draft blocks of 7 on 3k 88 us (97 sustained), 32 rows on 1k 30 us, one token on 1000 keys 12 us: what an item
+// costs beside its tiles (query parts, first wait, pieces and their merge).  At one clock and without gain: a warp each for
+// the score and the PV MMAs (the softmax then waits for P's buffer itself: 371 against 354 us), and 8 columns a
+// group for items of at most 16 (352 against 347 us: the chain is latency, not columns).
 #include "paged_items.cuh"
 #include "specdec_b200.h"
 

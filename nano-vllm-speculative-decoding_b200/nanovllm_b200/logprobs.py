@@ -77,8 +77,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, num_top: int = 0,
         tokens = tokens.to(torch.int64).contiguous()
     device = logits.device
     floats = torch.empty(T * (2 + num_top), dtype=torch.float32, device=device)      # one allocation for the three
-    out = TokenLogprobs(floats[:T], floats[T:2 * T], torch.empty(T, num_top, dtype=torch.int64, device=device),
-                        floats[2 * T:].view(T, num_top))
+    values, entropy, top = floats.split_with_sizes((T, T, T * num_top))
+    out = TokenLogprobs(values, entropy, torch.empty(T, num_top, dtype=torch.int64, device=device), top.view(T, num_top))
     base, dtype = floats.data_ptr(), DTYPE_CODES[logits.dtype]
     ws_bytes = _workspace_bytes(index, T, V, dtype, num_top)
     call_on(index, _lib.lib().specdec_token_logprobs, logits.data_ptr(), dtype, T, V, stride, tokens.data_ptr(),

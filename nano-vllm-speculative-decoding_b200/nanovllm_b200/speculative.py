@@ -200,8 +200,9 @@ class VerifyRound:
 
     def emitted_logprobs(self, num_tokens: int, drafts: torch.Tensor, n_accept: torch.Tensor, tail: torch.Tensor,
                          num_top: int = 0, verified_lens: torch.Tensor | None = None) -> TokenLogprobs:
-        """The last replay's log probabilities of the tokens that the round emitted: position j of a row's verified
-        tokens holds its emitted token j (accepted drafts, then the tail); later positions emitted none (0, ids -1)."""
+        """The last replay's log probabilities (of the model, at temperature 1) of the tokens that the round emitted:
+        position j of a row's verified tokens holds its emitted token j (accepted drafts, then the tail); later positions
+        emitted none (0, ids -1)."""
         num_verified, n, _ = self.loaded[num_tokens]
         k = drafts.shape[1]
         device = drafts.device

@@ -133,6 +133,47 @@ def test_rounds_on_the_device(varlen):
         assert np.array_equal(got.top_ids.cpu().numpy(), want[2])
 
 
+@pytest.mark.parametrize("varlen", [False, True])
+def test_host_and_device_rounds_agree(varlen):
+    """The same requests through run_round (host metadata, one copy back) and run_round_device: the same tokens, and the
+    same bytes in the caches, over rounds that cross block borders."""
+    from nanovllm_b200 import spec_sampler as S
+    host, dev = build(varlen), build(varlen)
+    R = len(host.lengths)
+    samp = S.sampling_tensors([SimpleNamespace(temperature=0.7, top_k=40, top_p=0.9)] * R, DEV)
+    gens = [torch.Generator(device=DEV).manual_seed(3) for _ in range(2)]
+    make = torch.Generator(device=DEV).manual_seed(4)
+    for step in range(3):
+        q = torch.softmax(torch.randn(R, K, host.shape.vocab, device=DEV, generator=make) * 0.3, -1)
+        drafts = S.sample(q, make)
+        lens = [1 + (5 * r + step) % (K + 1) for r in range(R)] if varlen else None
+        # the host side's blocks: those the device takes from its stack, in its order
+        have = host.rows.num_blocks.tolist()
+        free = int(host.rows.free_count)
+        for r, n in enumerate(host.rows.lengths.tolist()):
+            need = math.ceil((n - 1 + (lens[r] if varlen else K + 1)) / BS)
+            while have[r] < need:
+                free -= 1
+                host.rows.block_tables[r, have[r]] = host.rows.free_blocks[free]
+                have[r] += 1
+        host.rows.num_blocks.copy_(torch.tensor(have, dtype=torch.int32))
+        host.rows.free_count.fill_(free)
+        appended = host.rnd.run_round(host_rows(host.rows), drafts, q, samp, gens[0], lens)
+        n_accept, tail, none = dev.rnd.run_round_device(dev.rows, drafts, q, samp, gens[1],
+                                                        torch.tensor(lens, device=DEV) if varlen else None,
+                                                        sum(lens) if varlen else None)
+        assert none is None
+        assert appended == [drafts[r, :a].tolist() + [t] for r, (a, t) in enumerate(zip(n_accept.tolist(), tail.tolist()))]
+        host.rows.lengths.add_(torch.tensor([len(x) for x in appended], device=DEV))
+        host.rows.last_tokens.copy_(torch.tensor([x[-1] for x in appended], device=DEV))
+        for name in ("lengths", "last_tokens", "block_tables", "num_blocks", "free_count"):
+            assert torch.equal(getattr(host.rows, name), getattr(dev.rows, name)), name
+        for a, b in zip(host.target.kv_fp8, dev.target.kv_fp8):
+            assert torch.equal(a.k_scale, b.k_scale) and torch.equal(a.v_scale, b.v_scale)
+            assert torch.equal(a.k_cache.view(torch.uint8), b.k_cache.view(torch.uint8))
+            assert torch.equal(a.v_cache.view(torch.uint8), b.v_cache.view(torch.uint8))
+
+
 def test_a_round_without_blocks_leaves_the_rows():
     from nanovllm_b200 import device_metadata, logprobs
     from nanovllm_b200 import spec_sampler as S

@@ -74,26 +74,6 @@ __device__ __forceinline__ float column_reduce16(float (&v)[16], int lane) {
   return v[0];
 }
 
-// Sum over the 32 lanes of N (a power of two) columns held by every lane; lane j ends with column (j & (N - 1))'s sum.
-template <int N>
-__device__ __forceinline__ float column_reduce(float (&v)[N], int lane) {
-#pragma unroll
-  for (int w = 16; w >= N; w >>= 1)
-#pragma unroll
-    for (int c = 0; c < N; ++c) v[c] += __shfl_xor_sync(0xffffffffu, v[c], w);
-#pragma unroll
-  for (int w = N / 2; w >= 1; w >>= 1) {
-    const bool upper = (lane & w) != 0;
-#pragma unroll
-    for (int c = 0; c < w; ++c) {
-      const float send = upper ? v[c] : v[c + w];
-      const float keep = upper ? v[c + w] : v[c];
-      v[c] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-    }
-  }
-  return v[0];
-}
-
 // A row's queries and keys; nt = 0 when the row has no work (no queries, or metadata that the kernel rejects).
 struct RowInfo {
   int q_start, ql, L, nt;

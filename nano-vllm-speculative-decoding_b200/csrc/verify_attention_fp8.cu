@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       // ---- item epilogue: column sums over the 128 key threads, O^T out of TMEM
       if (live) {
-        const float s = column_reduce<kGroupCols>(l_part, lane);
+        const float s = column_reduce16(l_part, lane);
         if (lane < kGroupCols) S.red_sum[col][w] = s;
       }
       named_barrier(bar_wg, 128);

@@ -53,8 +53,9 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
   const long long length = a.lengths[r], n = a.verified_lens ? a.verified_lens[r] : a.k + 1;
   x.held = a.num_blocks[r];
   x.start = length - 1;
+  // the length against what the table leaves for the other tokens: their sum could pass 64 bits
   x.bad = n < 1 || n > a.k + 1 || length < 1 || x.held < 0 || x.held > a.table_width ||
-          length + n - 1 > (long long)a.table_width * a.block_size;
+          length > (long long)a.table_width * a.block_size - (n - 1);
   x.n = x.bad ? 0 : (int)n;
   if (x.bad) x.start = 0;
   x.need = (int)(((unsigned)(x.start + x.n) + (unsigned)a.block_size - 1u) / (unsigned)a.block_size);   // below 2^31 here

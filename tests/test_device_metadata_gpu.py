@@ -146,6 +146,25 @@ def test_bad_rows_and_a_dry_stack_assign_nothing(M, spoil, code):
     check(good, expected(s))
 
 
+@pytest.mark.parametrize("length", [2 ** 63 - 1, 2 ** 63 - 7, 2 ** 63 - 8, 2 ** 62, 2 ** 31, -2 ** 63, 4 * 128 - 6, 4 * 128 - 7])
+def test_lengths_up_to_the_type_s_end(M, length):
+    """A length whose sum with the row's 8 tokens wraps in 64 bits is refused like any other past the table's 6 blocks of 128
+    (of which width 4 are asked for); the longest that fits is served."""
+    s = case(6, 7, 128, 120, 128, 7, 4, 14, full=True)
+    d = on_device(s)
+    d["lengths"][2] = length
+    before = d["block_tables"].clone()
+    M.verify_metadata(**d)
+    v = packed_views(d["buf64"], d["buf32"], s["num_rows"], s["tokens"], s["width"])
+    if length == 4 * 128 - 7:
+        assert M.device_error(DEV) == 0
+        assert v["positions"][16:24].tolist() == list(range(4 * 128 - 8, 4 * 128)) and d["num_blocks"][2].item() == 4
+        return
+    assert M.device_error(DEV) == 7
+    M.reset_device_error(DEV)
+    assert torch.equal(before, d["block_tables"]) and (v["cu_seqlens_k"] == 0).all() and (v["slot_mapping"] == -1).all()
+
+
 def test_tokens_that_do_not_fit(M):
     s = case(6, 7, 128, 1, 300, 7, 4, 10)
     for tokens in (int(s["lens"].sum()) - 1, int(s["lens"].sum()) + 9):

@@ -301,12 +301,20 @@ int specdec_paged_attention_fp8(const void* q, long long T, long long q_row_stri
  * and *free_count lowered (both null: rows must hold what they need).  buf64 [2 num_tokens]: input ids, positions; buf32:
  * slot_mapping [num_tokens], cu_seqlens_q, cu_seqlens_k [num_rows + 1], block_tables [num_rows][width], padding rows of
  * at most k + 1 tokens on pad_block_id.  ticket: one zeroed word, left zero; calls sharing it must not overlap.  *err: 6
- * the stack ran out, 7 a row argument out of range; such a call assigns nothing and leaves every row empty. */
+ * the stack ran out, 7 a row argument out of range, 9 a needed block id, held or from the stack, negative or with slots
+ * past 32 bits; such a call assigns nothing (after 9, tables may differ past num_blocks) and leaves every row empty. */
 int specdec_verify_metadata(const long long* lengths, const long long* last_tokens, const long long* drafts,
                             const long long* verified_lens, int R, int k, int* block_tables, int table_width,
                             int* num_blocks, const int* free_blocks, int* free_count, int free_capacity,
                             int block_size, int num_rows, int num_tokens, int pad_block_id, int width,
                             long long* buf64, int* buf32, unsigned* ticket, int* err, void* stream);
+/* The same for a cache of cache_blocks blocks (0: any ids whose slots fit 32 bits): ids from there on are error 9 too. */
+int specdec_verify_metadata_ex(const long long* lengths, const long long* last_tokens, const long long* drafts,
+                               const long long* verified_lens, int R, int k, int* block_tables, int table_width,
+                               int* num_blocks, const int* free_blocks, int* free_count, int free_capacity,
+                               int block_size, int num_rows, int num_tokens, int pad_block_id, int width,
+                               long long* buf64, int* buf32, unsigned* ticket, int* err, long long cache_blocks,
+                               void* stream);
 
 /* ------------------------------------------------------------------------------------------ log probabilities */
 /* What a server answers with beside the tokens (probs_from_logits, nanovllm/layers/spec_sampler.py:65-69, writes all

@@ -14,9 +14,11 @@
 //
 // One launch, one warp a row.  Everything is a prefix over R rows of three numbers; a warp sums the rows before its own
 // straight from the inputs (a few loads a lane) instead of waiting for a scan of another block.  The rows' block counts
-// and the free count, which every warp reads, are written by the CTA that finishes last (a ticket that wraps itself).
-// Latency-bound: the loads' and the ticket's round trips.  64 rows take 4.3 us, 512 rows 7.1 us (a chain of array
-// operations on the GPU: 646 and 667 us).
+// and the free count, which every warp reads, are written by the CTA that finishes last (a ticket).  A block id outside the
+// cache is met only where a row's table is read; the ticket counts the CTAs that met one, and the last CTA empties the
+// metadata then instead of writing the counts.
+// Latency-bound: the loads' and the ticket's round trips.  64 rows of up to 64 blocks take 4.7 us, 512 rows 7.5 us
+// (4.6 and 7.1 without the check of the ids; a chain of array operations on the GPU: 646 and 667 us).
 #include "common.cuh"
 
 namespace specdec {
@@ -24,7 +26,8 @@ namespace metadata {
 
 constexpr int kThreads = 256;
 constexpr int kRowsPerCta = kThreads / 32;
-constexpr int kErrPool = 6, kErrRows = 7;
+constexpr int kErrPool = 6, kErrRows = 7, kErrBlock = 9;
+constexpr unsigned kSpoiled = 1u << 16;  // in the ticket, above the count of at most 65535 / kRowsPerCta + 1 CTAs
 
 struct Args {
   const long long* lengths;        // [R] tokens of each row, the last token included
@@ -36,6 +39,7 @@ struct Args {
   const int* free_blocks;          // [capacity] stack, top at *free_count - 1; null: rows hold what they need
   int* free_count;                 // [1], in place
   int R, k, table_width, capacity, block_size, num_rows, num_tokens, pad_block_id, width;
+  unsigned cache_blocks;           // ids of the rows' blocks are below it
   long long *input_ids, *positions;
   int *slots, *cu_q, *cu_k, *out_tables;
   unsigned* ticket;                // 0 between launches
@@ -69,8 +73,22 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a) {
-  __shared__ int last_cta;
+// Every row empty, every token padding: by the last CTA, over what the others wrote.  Not inlined: it has no part in the
+// registers of the path that every call takes (inlined, 512 rows took 9.4 us for 7.5).
+__device__ __noinline__ void clear(const Args& a) {
+  __threadfence();
+  if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrBlock);
+  for (int i = threadIdx.x; i <= a.num_rows; i += kThreads) a.cu_q[i] = a.cu_k[i] = 0;
+  for (int t = threadIdx.x; t < a.num_tokens; t += kThreads) {
+    a.positions[t] = 0;
+    a.input_ids[t] = 0;
+    a.slots[t] = -1;
+  }
+  for (long long i = threadIdx.x; i < (long long)a.num_rows * a.width; i += kThreads) a.out_tables[i] = a.pad_block_id;
+}
+
+__global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const __grid_constant__ Args a) {
+  __shared__ int last_cta, spoiled;
   const int lane = threadIdx.x & 31;
   const int r = blockIdx.x * kRowsPerCta + (threadIdx.x >> 5);
   // sums over the rows before r and over all rows: tokens, keys, new blocks
@@ -104,6 +122,7 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
   const bool dry = !bad && all_fresh > available;
   const bool idle = bad || dry;      // nothing is assigned or stored: every row empty
   if (idle && r == 0 && lane == 0) atomicCAS(a.err, 0, bad ? kErrRows : kErrPool);
+  bool bad_id = false;
   if (r < a.num_rows) {
     int first, n, kv;
     long long start = 0, k0;
@@ -132,11 +151,12 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
     // the row's table: what it holds, then its new blocks from the top of the stack, then the pad block
     int* out = a.out_tables + (long long)r * a.width;
     int* table = a.tables + (long long)r * a.table_width;
-    int held = 0, have = 0;
+    int held = 0, have = 0, need = 0;
     if (r < a.R && !idle) {
       const Row x = row_of(a, r);
       held = x.held;
-      have = max(x.held, x.need);
+      need = x.need;
+      have = max(held, need);
     }
     for (int j = lane; j < a.width; j += 32) {
       int b = a.pad_block_id;
@@ -146,6 +166,7 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
         b = a.free_blocks[available - 1 - (fresh + j - held)];
         table[j] = b;
       }
+      if (j < need && (unsigned)b >= a.cache_blocks) bad_id = true;
       out[j] = b;
     }
     __syncwarp();
@@ -155,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
       const bool real = r < a.R;
       a.positions[t] = pos;
       a.input_ids[t] = !real ? 0 : j == 0 ? a.last_tokens[r] : a.drafts ? a.drafts[(long long)r * a.k + j - 1] : 0;
-      a.slots[t] = real ? table[pos / bs] * a.block_size + (int)(pos % bs) : -1;
+      a.slots[t] = real ? (int)((unsigned)table[pos / bs] * bs + pos % bs) : -1;    // of a bad id: emptied by the last CTA
     }
   }
   if (idle)                           // no row has tokens: the whole token range is padding
@@ -165,13 +186,21 @@ __global__ void __launch_bounds__(kThreads) verify_metadata_kernel(const Args a)
       a.slots[t] = -1;
     }
   // ---- the last CTA to get here (every other has read the counts) writes the rows' block counts and the free count
-  __syncthreads();
+  const int any_bad = __syncthreads_or(bad_id);
   if (threadIdx.x == 0) {
     __threadfence();
-    last_cta = atomicInc(a.ticket, gridDim.x - 1) == gridDim.x - 1;
+    const unsigned mine = any_bad ? 1u + kSpoiled : 1u, all = atomicAdd(a.ticket, mine) + mine;
+    last_cta = all % kSpoiled == gridDim.x;
+    spoiled = all >= kSpoiled;
+    if (last_cta) *a.ticket = 0;
   }
   __syncthreads();
-  if (!last_cta || idle || !a.free_blocks) return;
+  if (!last_cta || idle) return;
+  if (spoiled) {
+    clear(a);
+    return;
+  }
+  if (!a.free_blocks) return;
   for (int i = threadIdx.x; i < a.R; i += kThreads) {
     const Row x = row_of(a, i);
     if (x.need > x.held) a.num_blocks[i] = x.need;
@@ -186,11 +215,12 @@ using namespace specdec;
 
 extern "C" {
 
-int specdec_verify_metadata(const long long* lengths, const long long* last_tokens, const long long* drafts,
-                            const long long* verified_lens, int R, int k, int* block_tables, int table_width,
-                            int* num_blocks, const int* free_blocks, int* free_count, int free_capacity,
-                            int block_size, int num_rows, int num_tokens, int pad_block_id, int width,
-                            long long* buf64, int* buf32, unsigned* ticket, int* err, void* stream) {
+int specdec_verify_metadata_ex(const long long* lengths, const long long* last_tokens, const long long* drafts,
+                               const long long* verified_lens, int R, int k, int* block_tables, int table_width,
+                               int* num_blocks, const int* free_blocks, int* free_count, int free_capacity,
+                               int block_size, int num_rows, int num_tokens, int pad_block_id, int width,
+                               long long* buf64, int* buf32, unsigned* ticket, int* err, long long cache_blocks,
+                               void* stream) {
   using namespace metadata;
   SPECDEC_CHECK_ARG(R >= 0 && num_rows >= R && num_rows >= 1 && num_rows <= 65535 && k >= 0 && k <= 1023,
                     "bad row sizes: %d of %d rows, %d drafts", R, num_rows, k);
@@ -201,6 +231,7 @@ int specdec_verify_metadata(const long long* lengths, const long long* last_toke
   SPECDEC_CHECK_ARG(R == 0 || (lengths && last_tokens && block_tables && num_blocks), "null row argument");
   SPECDEC_CHECK_ARG(!free_blocks == !free_count && free_capacity >= 0, "give free_blocks and free_count together");
   SPECDEC_CHECK_ARG(buf64 && buf32 && ticket && err, "null pointer argument");
+  SPECDEC_CHECK_ARG(cache_blocks >= 0 && cache_blocks <= 0x7fffffffLL / block_size, "the cache's slots must fit 32 bits");
   Args a{};
   a.lengths = lengths;
   a.last_tokens = last_tokens;
@@ -219,6 +250,7 @@ int specdec_verify_metadata(const long long* lengths, const long long* last_toke
   a.num_tokens = num_tokens;
   a.pad_block_id = pad_block_id;
   a.width = width;
+  a.cache_blocks = (unsigned)(cache_blocks ? cache_blocks : 0x7fffffffLL / block_size);
   a.input_ids = buf64;
   a.positions = buf64 + num_tokens;
   a.slots = buf32;
@@ -231,6 +263,16 @@ int specdec_verify_metadata(const long long* lengths, const long long* last_toke
   verify_metadata_kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
   SPECDEC_LAUNCH_CHECK();
   return kOk;
+}
+
+int specdec_verify_metadata(const long long* lengths, const long long* last_tokens, const long long* drafts,
+                            const long long* verified_lens, int R, int k, int* block_tables, int table_width,
+                            int* num_blocks, const int* free_blocks, int* free_count, int free_capacity,
+                            int block_size, int num_rows, int num_tokens, int pad_block_id, int width,
+                            long long* buf64, int* buf32, unsigned* ticket, int* err, void* stream) {
+  return specdec_verify_metadata_ex(lengths, last_tokens, drafts, verified_lens, R, k, block_tables, table_width, num_blocks,
+                                    free_blocks, free_count, free_capacity, block_size, num_rows, num_tokens, pad_block_id,
+                                    width, buf64, buf32, ticket, err, 0, stream);
 }
 
 }  // extern "C"

@@ -91,6 +91,9 @@ SIGNATURES = {
     "specdec_verify_metadata": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
                                          _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
                                          _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "specdec_verify_metadata_ex": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
+                                            _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                            _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_ll, _c_void_p]),
     "specdec_logprobs_workspace_bytes": (_c_ll, [_c_ll, _c_ll, _c_int, _c_int]),
     "specdec_token_logprobs": (_c_int, [_c_void_p, _c_int, _c_ll, _c_ll, _c_ll, _c_void_p, _c_void_p, _c_int,
                                         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_ll, _c_void_p,

@@ -2,7 +2,7 @@
 
     verify_metadata(...)    batch_metadata.pack_verify_metadata and draft_placement (nanovllm/engine/batch_metadata.py:
                             121-181, speculative.py:514-527) in one launch, the blocks that a row lacks taken from a free
-                            stack (scheduler.py:75-92)                                 -> specdec_verify_metadata
+                            stack (scheduler.py:75-92)                                 -> specdec_verify_metadata_ex
 
 The host form builds the arrays with numpy and copies them to the device three times a round; here the request state
 stays on the GPU (lengths, last tokens, drafts, block tables, the free blocks), so a round's metadata costs one launch and
@@ -50,8 +50,9 @@ def error_word(device: torch.device) -> torch.Tensor:
 def device_error(device: torch.device) -> int:
     """First error a verify_metadata call recorded on this device since the last reset (synchronises): 0 none, 6 the free
     blocks ran out, 7 row arguments out of range (a verified length outside 1..k+1, a length below 1, a table too narrow
-    for the row, tokens that the padding rows cannot hold).  A call that records one assigns nothing and leaves every row
-    empty: cumulative lengths 0, slots -1."""
+    for the row, tokens that the padding rows cannot hold), 9 a block that a row needs, held or from the stack, has an id
+    outside the cache.  A call that records one assigns nothing (num_blocks and free_count stay; after 9, block_tables may
+    differ past num_blocks) and leaves every row empty: cumulative lengths 0, slots -1."""
     return int(_words(device)[0].item())
 
 
@@ -67,7 +68,8 @@ def _of(name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple) -> 
 def verify_metadata(lengths: torch.Tensor, last_tokens: torch.Tensor, drafts: torch.Tensor,
                     verified_lens: torch.Tensor | None, block_tables: torch.Tensor, num_blocks: torch.Tensor,
                     free_blocks: torch.Tensor | None, free_count: torch.Tensor | None, *, block_size: int, num_rows: int,
-                    num_tokens: int, pad_block_id: int, width: int, buf64: torch.Tensor, buf32: torch.Tensor) -> None:
+                    num_tokens: int, pad_block_id: int, width: int, buf64: torch.Tensor, buf32: torch.Tensor,
+                    cache_blocks: int | None = None) -> None:
     """Writes the metadata of verifying R rows into the packed buffers buf64 / buf32 (batch_metadata.packed_views of
     num_rows, num_tokens and width names their parts), the drafts placed among the input ids.
 
@@ -76,7 +78,8 @@ def verify_metadata(lengths: torch.Tensor, last_tokens: torch.Tensor, drafts: to
     padding rows (at most k + 1 each) make num_tokens.  block_tables [R, W'] int32 and num_blocks [R] int32: the blocks a
     row holds, extended in place to what lengths - 1 + verified_lens tokens need with blocks from the top of the stack
     free_blocks[:free_count] (int32, free_count [1] int32, lowered in place), rows in order.  Both None: the rows must
-    hold what they need.  The row arguments may be empty (R = 0): all padding.  Calls on one device share an error word and
+    hold what they need.  cache_blocks: ids of the rows' blocks are below it (None: any whose slots fit 32 bits).  The row
+    arguments may be empty (R = 0): all padding.  Calls on one device share an error word and
     a ticket: they must not overlap on the GPU."""
     index = buf64.get_device()
     if not same_device(index, lengths, last_tokens, drafts, verified_lens, block_tables, num_blocks, free_blocks,
@@ -101,11 +104,13 @@ def verify_metadata(lengths: torch.Tensor, last_tokens: torch.Tensor, drafts: to
         capacity = free_blocks.numel()
         _of("free_blocks", free_blocks, torch.int32, (capacity,))
         _of("free_count", free_count, torch.int32, (1,))
+    if cache_blocks is not None and cache_blocks < 1:
+        raise ValueError(f"cache_blocks {cache_blocks}: the cache's blocks, or None")
     n64, n32 = packed_sizes(num_rows, num_tokens, width)
     _of("buf64", buf64, torch.int64, (n64,))
     _of("buf32", buf32, torch.int32, (n32,))
     words = Workspace.address(index, 256, "device_metadata")       # [error word, ticket]
-    call_on(index, _lib.lib().specdec_verify_metadata, ptr(lengths), ptr(last_tokens), ptr(drafts), ptr(verified_lens), R,
+    call_on(index, _lib.lib().specdec_verify_metadata_ex, ptr(lengths), ptr(last_tokens), ptr(drafts), ptr(verified_lens), R,
             k, ptr(block_tables), table_width, ptr(num_blocks), ptr(free_blocks), ptr(free_count), capacity, block_size,
             num_rows, num_tokens, pad_block_id, width, buf64.data_ptr(), buf32.data_ptr(), words + 4, words,
-            raw_stream(index))
+            0 if cache_blocks is None else cache_blocks, raw_stream(index))

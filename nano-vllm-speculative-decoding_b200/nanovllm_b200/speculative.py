@@ -157,7 +157,7 @@ class VerifyRound:
         verify_metadata(rows.lengths, rows.last_tokens, drafts, verified_lens, rows.block_tables, rows.num_blocks,
                         rows.free_blocks, rows.free_count, block_size=self.block_size, num_rows=self.shapes[num_tokens],
                         num_tokens=num_tokens, pad_block_id=self.target.pad_block_id, width=self.max_num_blocks,
-                        buf64=b["_packed64"], buf32=b["_packed32"])
+                        buf64=b["_packed64"], buf32=b["_packed32"], cache_blocks=self.target.num_blocks)
         self.loaded[num_tokens] = (num_verified, n, -1)
         self.device_lens[num_tokens] = verified_lens
         return num_tokens

@@ -165,6 +165,47 @@ def test_lengths_up_to_the_type_s_end(M, length):
     assert torch.equal(before, d["block_tables"]) and (v["cu_seqlens_k"] == 0).all() and (v["slot_mapping"] == -1).all()
 
 
+@pytest.mark.parametrize("where", ["held", "stack"])
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 2 ** 31 - 1, 2 ** 27, "cache"])
+def test_block_ids_outside_the_cache_assign_nothing(M, where, bad):
+    """One id among 40 rows that is negative, whose slots pass 32 bits, or that the cache does not have: nothing is assigned
+    and every row is empty, also with the ids of other rows good.  An id that no row needs does not matter."""
+    s = case(40, 7, 16, 100, 700, 44, 45, 15, full=True, fill=0.5)
+    blocks = s["pad"] if bad == "cache" else None
+    d = on_device(s)
+    d["cache_blocks"] = blocks
+    grown = int((s["need"] - s["held"]).sum())
+    assert 8 <= grown < len(s["free"])
+    d["free_blocks"][len(s["free"]) - grown - 1] = -5          # below what this call takes
+    d["block_tables"][3, int(s["held"][3]):] = -9              # past what row 3 holds
+    M.verify_metadata(**{**d, **{n: d[n].clone() for n in ("block_tables", "num_blocks", "free_count", "buf64", "buf32")}})
+    assert M.device_error(DEV) == 0
+    value = s["pad"] if bad == "cache" else bad
+    if where == "held":
+        r = int(np.argmax(s["held"] > 1))
+        d["block_tables"][r, 1] = value
+    else:
+        d["free_blocks"][len(s["free"]) - 7] = value
+    state = {n: d[n].clone() for n in ("num_blocks", "free_count", "free_blocks")}
+    held_blocks = lambda t: t[torch.arange(t.shape[1], device=DEV) < d["num_blocks"][:, None]]  # noqa: E731
+    before = held_blocks(d["block_tables"])
+    for _ in range(2):                                         # the ticket is left as it was found
+        M.verify_metadata(**d)
+        assert M.device_error(DEV) == 9
+        M.reset_device_error(DEV)
+        assert all(torch.equal(state[n], d[n]) for n in state)
+        assert torch.equal(held_blocks(d["block_tables"]), before)
+        v = packed_views(d["buf64"], d["buf32"], s["num_rows"], s["tokens"], s["width"])
+        assert (v["cu_seqlens_q"] == 0).all() and (v["cu_seqlens_k"] == 0).all() and (v["slot_mapping"] == -1).all()
+        assert (v["block_tables"] == s["pad"]).all() and (v["input_ids"] == 0).all() and (v["positions"] == 0).all()
+    good = on_device(s)                    # the next call is untouched by it
+    M.verify_metadata(**good, cache_blocks=s["pad"])
+    assert M.device_error(DEV) == 0
+    check(good, expected(s))
+    with pytest.raises(ValueError, match="cache_blocks"):
+        M.verify_metadata(**good, cache_blocks=0)
+
+
 def test_tokens_that_do_not_fit(M):
     s = case(6, 7, 128, 1, 300, 7, 4, 10)
     for tokens in (int(s["lens"].sum()) - 1, int(s["lens"].sum()) + 9):

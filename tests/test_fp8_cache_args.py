@@ -72,6 +72,13 @@ def test_metadata_refuses(lib, bad, message):
     assert message in lib.specdec_last_error()
 
 
+@pytest.mark.parametrize("blocks", [-1, 2 ** 31 // 256, 2 ** 40])
+def test_metadata_refuses_a_cache_past_32_bits(lib, blocks):
+    args = metadata_args()
+    assert lib.specdec_verify_metadata_ex(*args[:-1], blocks, args[-1]) == 1
+    assert b"32 bits" in lib.specdec_last_error()
+
+
 def logprob_args(**kw):
     a = dict(x=FAKE, dtype=1, T=8, V=1000, stride=1000, tokens=FAKE, temps=None, top=5, lp=FAKE, ent=FAKE, ids=FAKE, tlp=FAKE,
              ws=FAKE, wsb=1 << 30, err=FAKE, stream=None)

@@ -219,6 +219,36 @@ def test_a_round_without_blocks_leaves_the_rows():
         logprobs.reset_device_error(DEV)
 
 
+@pytest.mark.parametrize("where", ["table", "stack"])
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 10 ** 6, 2 ** 30, 2 ** 24, "pad"])
+def test_bad_block_ids_hold_the_rows(where, bad):
+    """An id that the target's cache does not have, in a row's table or on the stack: error 9, nothing stored, no row
+    moved."""
+    from nanovllm_b200 import attention, device_metadata
+    from nanovllm_b200 import spec_sampler as S
+    c = build(False)
+    R = len(c.lengths)
+    samp = S.sampling_tensors([SimpleNamespace(temperature=0.0, top_k=0, top_p=1.0)] * R, DEV)
+    drafts = torch.randint(c.shape.vocab, (R, K), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    bad = c.target.pad_block_id if bad == "pad" else bad
+    if where == "table":
+        c.rows.block_tables[2, 0] = bad
+    else:
+        c.rows.free_blocks[int(c.rows.free_count) - 1] = bad
+    before = [t.clone() for t in (c.rows.lengths, c.rows.last_tokens, c.rows.num_blocks, c.rows.free_count)]
+    caches = [(l.k_cache.view(torch.uint8).clone(), l.v_cache.view(torch.uint8).clone()) for l in c.target.kv_fp8]
+    try:
+        c.rnd.run_round_device(c.rows, drafts, None, samp)
+        assert device_metadata.device_error(DEV) == 9 and attention.device_error(DEV) == 0
+        after = (c.rows.lengths, c.rows.last_tokens, c.rows.num_blocks, c.rows.free_count)
+        assert all(torch.equal(x, y) for x, y in zip(before, after))
+        for (k, v), l in zip(caches, c.target.kv_fp8):
+            assert torch.equal(k, l.k_cache.view(torch.uint8)) and torch.equal(v, l.v_cache.view(torch.uint8))
+    finally:
+        device_metadata.reset_device_error(DEV)
+        attention.reset_device_error(DEV)
+
+
 def test_greedy_rounds_of_a_padded_batch():
     """Fewer rows than the graph has, all greedy: the emitted tokens follow the argmax of the round's own logits."""
     from nanovllm_b200 import device_metadata

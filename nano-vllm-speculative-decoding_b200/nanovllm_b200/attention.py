@@ -32,8 +32,13 @@ def _err_word(device: torch.device) -> torch.Tensor:
 def device_error(device: torch.device) -> int:
     """First error code a paged-attention / K-V store kernel recorded on this device since the last reset
     (synchronises): 0 none, 2 row metadata inconsistent with the block table width, 3 a slot past the cache,
-    11-17 a bounded pipeline wait gave up."""
+    5 a block id outside the 8-bit cache, 11-17 a bounded pipeline wait gave up."""
     return int(_err_word(device).item())
+
+
+def error_word(device: torch.device) -> torch.Tensor:
+    """The int32 word that device_error reads, on the device."""
+    return _err_word(device)[0]
 
 
 def reset_device_error(device: torch.device) -> None:

@@ -19,6 +19,17 @@ def err_word(device: torch.device) -> torch.Tensor:
     return Workspace.get(device, 256, name="fused")[:4].view(torch.int32)
 
 
+def device_error(device: torch.device) -> int:
+    """First error recorded on this device since the last reset by the kernels that share this word: those here, the Markov
+    rows and the context store (synchronises): 0 none, 3 a slot past the cache, 4 a position outside the rotary table,
+    others a bounded wait that gave up."""
+    return int(err_word(device).item())
+
+
+def reset_device_error(device: torch.device) -> None:
+    err_word(device).zero_()
+
+
 def rope_cache(head_dim: int, max_position: int, base: float, device: torch.device) -> torch.Tensor:
     """rotary_embedding.py:17-27: [max_position, head_dim] fp32 = cat(cos(t * inv_freq), sin(t * inv_freq))."""
     inv_freq = 1.0 / (base ** (torch.arange(0, head_dim, 2, dtype=torch.float) / head_dim))

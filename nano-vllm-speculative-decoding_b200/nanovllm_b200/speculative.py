@@ -23,7 +23,7 @@ from collections import Counter
 import numpy as np
 import torch
 
-from . import spec_sampler
+from . import attention, fused, spec_sampler
 from .batch_metadata import (RowState, draft_packed_sizes, draft_packed_views, draft_placement,
                              pack_draft_block_metadata, pack_verify_metadata)
 from .device_metadata import DeviceRows, error_word, verify_metadata
@@ -227,14 +227,18 @@ class VerifyRound:
                          num_top: int | None = None) -> tuple[torch.Tensor, torch.Tensor, TokenLogprobs | None]:
         """run_round with the requests on the GPU and no host copy in either direction: returns n_accept [R], tail [R]
         and, with num_top, the emitted tokens' log probabilities (emitted_logprobs); rows are advanced.  Where the
-        metadata recorded an error (device_metadata.device_error: the free blocks ran out, lengths out of range) the round
-        has stored nothing, its results are void and the rows stay as they were, until the error is reset; where the
-        acceptance refused its inputs, lengths of another sum than num_verified say, they stay for this round."""
+        metadata recorded an error (device_metadata.device_error: the free blocks ran out, lengths or block ids out of
+        range) the round has stored nothing, its results are void and the rows stay as they were, until the error is
+        reset.  They stay until the reset, too, where the forward recorded one (fused.device_error: a position past the
+        target's last; attention.device_error): logits may be void then.  Where the acceptance refused its inputs, lengths
+        of another sum than num_verified say, they stay for this round."""
         num_tokens = self.load_device(rows, drafts, verified_lens, num_verified)
         n_accept, tail = self.verify_and_accept(num_tokens, drafts.shape[0], drafts, draft_probs, sampling, generator)
         logprobs = (None if num_top is None else
                     self.emitted_logprobs(num_tokens, drafts, n_accept, tail, num_top, verified_lens))
-        rows.advance(n_accept, tail, error_word(drafts.device) | spec_sampler.status_word(drafts.device))
+        device = drafts.device
+        rows.advance(n_accept, tail, error_word(device) | fused.err_word(device)[0] | attention.error_word(device)
+                     | spec_sampler.status_word(device))
         return n_accept, tail, logprobs
 
     def commit(self, drafts: torch.Tensor, n_accept: torch.Tensor, tail: torch.Tensor,

@@ -249,6 +249,53 @@ def test_bad_block_ids_hold_the_rows(where, bad):
         attention.reset_device_error(DEV)
 
 
+@pytest.mark.parametrize("module", ["attention", "fused"])
+def test_errors_of_the_forward_hold_the_rows(module):
+    """With an error word of the forward's kernels set, a round moves no row; after the reset it does."""
+    import importlib
+    from nanovllm_b200 import spec_sampler as S
+    m = importlib.import_module(f"nanovllm_b200.{module}")
+    assert m.device_error(DEV) == 0
+    c = build(False)
+    R = len(c.lengths)
+    samp = S.sampling_tensors([SimpleNamespace(temperature=0.0, top_k=0, top_p=1.0)] * R, DEV)
+    drafts = torch.randint(c.shape.vocab, (R, K), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    before = (c.rows.lengths.clone(), c.rows.last_tokens.clone())
+    try:
+        (m.error_word(DEV) if module == "attention" else m.err_word(DEV)).fill_(4)
+        c.rnd.run_round_device(c.rows, drafts, None, samp)
+        assert torch.equal(c.rows.lengths, before[0]) and torch.equal(c.rows.last_tokens, before[1])
+    finally:
+        m.reset_device_error(DEV)
+    n_accept, tail, _ = c.rnd.run_round_device(c.rows, drafts, None, samp)
+    assert torch.equal(c.rows.lengths, before[0] + n_accept + 1) and torch.equal(c.rows.last_tokens, tail)
+
+
+def test_a_row_past_the_last_position_holds_the_rows():
+    """A row whose drafts cross the rotary table's end (its tokens there are neither rotated nor stored): error 4."""
+    from nanovllm_b200 import attention, device_metadata, fused
+    from nanovllm_b200 import spec_sampler as S
+    c = build(False)
+    R = len(c.lengths)
+    samp = S.sampling_tensors([SimpleNamespace(temperature=0.0, top_k=0, top_p=1.0)] * R, DEV)
+    drafts = torch.randint(c.shape.vocab, (R, K), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    end = 513 + 3                             # row 2 verifies positions 512 to 519
+    c.target.cos_sin = c.target.cos_sin[:end]
+    c.target.graphs.clear()
+    c.target.graph_pool = None
+    from nanovllm_b200.speculative import VerifyRound
+    rnd = VerifyRound(c.target, K, [R], 4)
+    assert fused.device_error(DEV) == 0
+    before = (c.rows.lengths.clone(), c.rows.last_tokens.clone())
+    try:
+        rnd.run_round_device(c.rows, drafts, None, samp)
+        assert fused.device_error(DEV) == 4
+        assert device_metadata.device_error(DEV) == 0 and attention.device_error(DEV) == 0
+        assert torch.equal(c.rows.lengths, before[0]) and torch.equal(c.rows.last_tokens, before[1])
+    finally:
+        fused.reset_device_error(DEV)
+
+
 def test_greedy_rounds_of_a_padded_batch():
     """Fewer rows than the graph has, all greedy: the emitted tokens follow the argmax of the round's own logits."""
     from nanovllm_b200 import device_metadata

@@ -97,7 +97,13 @@ __global__ void __launch_bounds__(256) norm_rope_store_kernel(const NormRopeArgs
   const int hh = (int)(item % heads);
   const long long pos = a.positions[t];
   if (pos < 0 || pos >= a.max_position) {
+    // nothing is stored, and the query is zero: the row's other queries share an exponent with it in the 8-bit cache's
+    // attention, which memory as it was found would spoil
     if (lane == 0) atomicCAS(a.err, 0, 4);
+    if (hh < a.Hq) {
+      const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      store_head(a.q_out + ((long long)t * a.Hq + hh) * kHeadDim, lane, zero);
+    }
     return;
   }
   const float* cs = a.cos_sin + pos * kHeadDim;

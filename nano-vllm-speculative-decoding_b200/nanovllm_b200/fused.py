@@ -5,6 +5,7 @@
     qk_norm_rope_store(...)                 nanovllm/models/qwen3.py:77-86 + attention.py:62-63
                                             (q_norm, k_norm, RoPE, store_kvcache in one launch) -> specdec_norm_rope_store
     qk_norm_rope(...)                       the same without the cache: q, k, v rows in token order
+    slots_in_range(...)                     the slots of the tokens that qk_norm_rope writes, -1 for the others
     rope_cache(head_dim, max_position, base) nanovllm/layers/rotary_embedding.py:17-27 (the cos|sin table)
 """
 from __future__ import annotations
@@ -68,7 +69,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, q_n
                        slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, eps: float,
                        q_out: torch.Tensor | None = None) -> torch.Tensor:
     """The verify forward's qkv [T, (H + 2 Hkv) * 128] -> q [T, H, 128] (q_norm, RoPE); k_norm + RoPE'd K and V
-    rows go straight to their slots of the layer's paged caches (slot -1 skipped)."""
+    rows go straight to their slots of the layer's paged caches (slot -1 skipped).  A token whose position lies outside
+    cos_sin is not stored and has a zero query (device_error 4)."""
     device = require_cuda(qkv, positions, slot_mapping, k_cache, v_cache)
     T = qkv.shape[0]
     head_dim = 128
@@ -86,7 +88,15 @@ def qk_norm_rope(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, q_norm: t
                  cos_sin: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, eps: float
                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """qk_norm_rope_store with the K and V rows kept in token order instead of a cache's slots (for a store of another
-    format): q [T, H, 128], k and v [T, Hkv, 128].  rows: int32 0 .. T-1 on the device."""
+    format): q [T, H, 128], k and v [T, Hkv, 128].  rows: int32 0 .. T-1 on the device.  A token whose position lies outside
+    cos_sin has a zero query, and its K and V rows left unwritten (error 4) as qk_norm_rope_store leaves its slot: store with
+    slots_in_range."""
     k, v = (torch.empty(qkv.shape[0], num_kv_heads, 128, dtype=qkv.dtype, device=qkv.device) for _ in range(2))
     q = qk_norm_rope_store(qkv, num_heads, num_kv_heads, q_norm, k_norm, cos_sin, positions, rows, k, v, eps)
     return q, k, v
+
+
+def slots_in_range(slot_mapping: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor) -> torch.Tensor:
+    """slot_mapping with -1 for the tokens whose position lies outside cos_sin: qk_norm_rope writes no row for them, and
+    what their slots would get (memory as it was found) could raise the scale of a group that holds other tokens."""
+    return slot_mapping.masked_fill(positions.clamp(0, cos_sin.shape[0] - 1) != positions, -1)

@@ -122,12 +122,13 @@ class Qwen3Target:
         store = None
         if self.kv_fp8 is not None:
             rows = torch.arange(input_ids.shape[0], dtype=torch.int32, device=self.device)
+            slots = fused.slots_in_range(slot_mapping, positions, self.cos_sin)
 
             def store(qkv, w, layer_id):
                 c = self.kv_fp8[layer_id]
                 q, k, v = fused.qk_norm_rope(qkv, s.heads, s.kv_heads, w["q_norm"], w["k_norm"], self.cos_sin, positions,
                                              rows, s.eps)
-                store_kvcache_fp8(k, v, c.k_cache, c.v_cache, c.k_scale, c.v_scale, slot_mapping)
+                store_kvcache_fp8(k, v, c.k_cache, c.v_cache, c.k_scale, c.v_scale, slots)
                 return q
 
         def attend(q, layer_id):

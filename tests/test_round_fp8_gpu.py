@@ -271,6 +271,47 @@ def test_errors_of_the_forward_hold_the_rows(module):
     assert torch.equal(c.rows.lengths, before[0] + n_accept + 1) and torch.equal(c.rows.last_tokens, tail)
 
 
+def poison(value=1e30):
+    """Freed memory that torch.empty hands out next holds large values, small and large blocks alike."""
+    junk = [torch.full((n,), value, dtype=torch.bfloat16, device=DEV) for n in [2048] * 500 + [1 << 22] * 4]
+    torch.cuda.synchronize()
+    del junk
+
+
+def test_tokens_past_the_last_position_store_nothing():
+    """Rows 259 to 266 of a target whose rotary table ends at 264: the caches' bytes are those of a forward that gives the last
+    three tokens no slot, group mates of theirs included (memory that the forward finds holds 1e30)."""
+    from nanovllm_b200 import fused
+    from nanovllm_b200.attention_fp8 import store_kvcache_fp8
+    from nanovllm_b200.target import Qwen3Shape, Qwen3Target
+    shape = Qwen3Shape(hidden=256, layers=2, heads=4, kv_heads=2, intermediate=512, vocab=1000, max_position=264)
+    tables = torch.tensor([[1, 2]], dtype=torch.int32, device=DEV)
+    ids = torch.arange(8, device=DEV)
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device=DEV) for n in (8, 267))
+    at = torch.arange(259, 267, device=DEV)
+    slots = (tables[0, at // BS] * BS + at % BS).to(torch.int32)
+    caches = []
+    for given in (True, False):
+        target = Qwen3Target(shape, DEV, 3, BS, seed=5, init_scale=0.05, kv_dtype=torch.float8_e4m3fn)
+        g = torch.Generator(device=DEV).manual_seed(2)
+        for c in target.kv_fp8:
+            pos = torch.arange(259, device=DEV)
+            x = torch.randn(2, 259, 2, 128, device=DEV, generator=g).bfloat16()
+            store_kvcache_fp8(x[0], x[1], c.k_cache, c.v_cache, c.k_scale, c.v_scale,
+                              (tables[0, pos // BS] * BS + pos % BS).to(torch.int32))
+        poison()
+        inside = at < 264
+        target.forward(ids, at if given else torch.where(inside, at, 0),
+                       slots if given else torch.where(inside, slots, -1).to(torch.int32), cu_q, cu_k, 8, tables)
+        torch.cuda.synchronize()
+        caches.append([t.clone() for c in target.kv_fp8 for t in (c.k_cache.view(torch.uint8), c.v_cache.view(torch.uint8),
+                                                                  c.k_scale, c.v_scale)])
+    code = fused.device_error(DEV)
+    fused.reset_device_error(DEV)
+    assert code == 4
+    assert all(torch.equal(a, b) for a, b in zip(*caches))
+
+
 def test_a_row_past_the_last_position_holds_the_rows():
     """A row whose drafts cross the rotary table's end (its tokens there are neither rotated nor stored): error 4."""
     from nanovllm_b200 import attention, device_metadata, fused

@@ -30,6 +30,10 @@ const char* specdec_last_error(void);
 int specdec_version(void);
 /* 1 when the current CUDA device is compute capability 10.0 (the only target of this build). */
 int specdec_device_supported(void);
+/* Sets the calling thread's stream-capture mode (0 global, 1 thread-local, 2 relaxed) and returns the one before, -1 on an
+ * error.  For a caller that has to allocate and fill a workspace while a stream of it is being captured: relaxed around
+ * that, the old mode after. */
+int specdec_exchange_capture_mode(int mode);
 
 /* ------------------------------------------------------------------------------------------ kernel 1: sampler */
 /* Workspace bytes for the sampler entry points over `rows` rows of logits / probabilities (no counterpart in the

@@ -53,4 +53,20 @@ int specdec_device_supported(void) {
   return info.cc_major == 10 && info.cc_minor == 0;
 }
 
+// See the header: the mode before, or -1.
+int specdec_exchange_capture_mode(int mode) {
+  if (mode < 0 || mode > 2) {
+    specdec::set_error(specdec::kInvalidArgument, "capture mode %d: 0 global, 1 thread-local, 2 relaxed", mode);
+    return -1;
+  }
+  static_assert(cudaStreamCaptureModeGlobal == 0 && cudaStreamCaptureModeThreadLocal == 1 && cudaStreamCaptureModeRelaxed == 2);
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(mode);
+  const cudaError_t err = cudaThreadExchangeStreamCaptureMode(&m);
+  if (err != cudaSuccess) {
+    specdec::set_error(specdec::kCudaError, "cudaThreadExchangeStreamCaptureMode failed: %s", cudaGetErrorString(err));
+    return -1;
+  }
+  return static_cast<int>(m);
+}
+
 }  // extern "C"

@@ -91,6 +91,7 @@ SIGNATURES = {
     "specdec_verify_metadata": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
                                          _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
                                          _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "specdec_exchange_capture_mode": (_c_int, [_c_int]),
     "specdec_verify_metadata_ex": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
                                             _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
                                             _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_ll, _c_void_p]),
@@ -189,7 +190,9 @@ def call_on(index: int, function, *args) -> None:
 
 class Workspace:
     """A zero-initialised device byte buffer per (device, name), grown on demand.  The library keeps its tickets
-    and argmax keys self-cleaning at fixed offsets, so the buffer is zeroed once per allocation only.  A grown
+    and argmax keys self-cleaning at fixed offsets, so the buffer is zeroed once per allocation only, and at once: before
+    get returns, on a stream of its own, also while the current stream is being captured.  (A fill left to the capture
+    would run only with that graph's replays, not for calls and graphs that use the buffer before them.)  A grown
     buffer's predecessor is kept alive: a CUDA graph captured with the old address keeps replaying into valid
     memory (its own, since later calls outside the graph use the new buffer)."""
 
@@ -212,8 +215,24 @@ class Workspace:
             if buf is not None:
                 cls._retired.append(buf)
             size = max(nbytes, 1 << 20)
-            buf = torch.zeros(size, dtype=torch.uint8, device=device)
+            buf = cls._zeroed(size, device)
             cls._buffers[key] = buf
+        return buf
+
+    @staticmethod
+    def _zeroed(size: int, device: torch.device) -> torch.Tensor:
+        if device.type != "cuda":
+            return torch.zeros(size, dtype=torch.uint8, device=device)
+        mode = lib().specdec_exchange_capture_mode(2)       # relaxed: a capture forbids this thread allocations and waits
+        if mode < 0:
+            raise SpecdecError(lib().specdec_last_error().decode(errors="replace"))
+        try:
+            stream = torch.cuda.Stream(device)
+            with torch.cuda.stream(stream):
+                buf = torch.zeros(size, dtype=torch.uint8, device=device)
+            stream.synchronize()
+        finally:
+            lib().specdec_exchange_capture_mode(mode)
         return buf
 
 

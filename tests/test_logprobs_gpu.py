@@ -143,3 +143,35 @@ def test_no_rows_and_refusals(P):
                 (x, tokens, 1, torch.ones(3, device=DEV))):
         with pytest.raises(ValueError):
             P.token_logprobs(*bad)
+
+
+def test_a_workspace_first_used_in_a_capture(P):
+    """A workspace that a captured call is the first to name is zero from then on, not from that graph's first replay: in
+    memory of the graphs' pool that held other data, a second graph and an eager call give the same numbers before it."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn(2, 150000, device=DEV, generator=g)
+    tokens = torch.tensor([3, 5], device=DEV)
+    want = P.token_logprobs(x, tokens, 4)
+    pool = torch.cuda.graph_pool_handle()
+    dirty = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(dirty, pool):
+        junk = [torch.full((1 << 20,), 0x5A, dtype=torch.uint8, device=DEV) for _ in range(8)]
+    dirty.replay()
+    torch.cuda.synchronize()
+    del junk
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool):
+            outs.append(P.token_logprobs(x, tokens, 4, workspace="logprobs_first_in_a_capture"))
+        graphs.append(graph)
+    eager = P.token_logprobs(x, tokens, 4, workspace="logprobs_first_in_a_capture")
+    for n in (1, 0, 1):
+        for t in (outs[n].logprobs, outs[n].entropy, outs[n].top_ids, outs[n].top_logprobs):
+            t.fill_(7)
+        graphs[n].replay()
+        torch.cuda.synchronize()
+        for got in (outs[n], eager):
+            for a, b in ((got.logprobs, want.logprobs), (got.entropy, want.entropy), (got.top_ids, want.top_ids),
+                         (got.top_logprobs, want.top_logprobs)):
+                assert torch.equal(a, b)

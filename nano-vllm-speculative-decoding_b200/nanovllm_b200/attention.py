@@ -94,6 +94,11 @@ def _row_metadata(block_tables, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, contex
     return tables, None, None, ctx, ctx.numel(), query_len_per_seq, query_len_per_seq
 
 
+def given_as_is(*pairs) -> bool:
+    """Whether every (used, given) pair is one tensor: none was converted (used None: not read)."""
+    return all(used is None or used is given for used, given in pairs)
+
+
 def _output(out: torch.Tensor | None, shape, device: torch.device) -> torch.Tensor:
     """out itself after checking it is a bf16 [T, H, D] tensor on `device` with dense heads (rows may be strided),
     or a new one."""
@@ -116,7 +121,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of q [T, H, D] over the paged caches.  Varlen (cu_seqlens_q/k, the verify forward) or decode
     (context_lens with query_len_per_seq queries per row).  Returns out [T, H, D] bf16.  early_launch: launch as a
     programmatic dependent of the preceding kernel (its prologue overlaps that kernel's end); only when that kernel
-    does not write the row metadata (cu_seqlens / context_lens / block_tables).  max_ctas (1..255, 0 = one per SM):
+    does not write the row metadata (cu_seqlens / context_lens / block_tables); without effect where these have to be
+    converted to dense int32 first, since the conversion is that kernel then.  max_ctas (1..255, 0 = one per SM):
     cap the persistent grid, leaving SMs to work on another stream.  workspace: the name of the split-item
     workspace; launches that may run at the same time on different streams need different names."""
     device = require_cuda(q, k_cache, v_cache, block_tables)
@@ -152,6 +158,8 @@ def paged_attention_to(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     if not 0 <= max_ctas <= 255:
         raise ValueError(f"max_ctas {max_ctas}: 0 (one CTA per SM) to 255")
     ws = _split_workspace(device, R, Hkv, workspace)
+    early_launch = early_launch and given_as_is((tables, block_tables), (cq, cu_seqlens_q), (ck, cu_seqlens_k),
+                                                (ctx, context_lens))
     flags = (EARLY_LAUNCH if early_launch else 0) | (max_ctas << CTAS_SHIFT)
     if len(out_ptrs) == 1:
         check(_lib.lib().specdec_paged_attention_ex(

@@ -36,7 +36,7 @@ import torch
 
 from . import _lib
 from ._lib import Workspace, call_on, ptr, raw_stream, require_cuda, same_device
-from .attention import _SPLIT_MIN_BYTES, CTAS_SHIFT, EARLY_LAUNCH, _output
+from .attention import _SPLIT_MIN_BYTES, CTAS_SHIFT, EARLY_LAUNCH, _output, given_as_is
 from .context import get_context
 
 HEAD_DIM = 128
@@ -178,6 +178,8 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         q = q.contiguous()
         strides = q.stride()
     ws_bytes = _workspace_bytes(index, R, kv_heads)
+    early_launch = early_launch and given_as_is((tables, block_tables), (cq, cu_seqlens_q), (ck, cu_seqlens_k),
+                                                (ctx, context_lens))
     flags = (EARLY_LAUNCH if early_launch else 0) | (max_ctas << CTAS_SHIFT)
     call_on(index, _lib.lib().specdec_paged_attention_fp8, q.data_ptr(), T, strides[0], H, kv_heads, D,
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size, group,

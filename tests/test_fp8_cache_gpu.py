@@ -371,6 +371,44 @@ def test_attention_in_graphs_and_on_another_stream(F):
     assert device_error() == 0
 
 
+@pytest.mark.parametrize("cache", ["e4m3", "bf16"])
+def test_early_launch_only_on_metadata_given_as_int32(F, cache, monkeypatch):
+    """An early launch reads the row metadata before the kernel in front of it has ended, so it must not follow a conversion
+    of them: int64 (or strided) metadata launch in order.  The flags are those that reach the library."""
+    from nanovllm_b200 import _lib, attention
+    flags = []
+    real = _lib.lib()
+
+    class Recorder:
+        def __getattr__(self, name):
+            fn = getattr(real, name)
+            if name not in ("specdec_paged_attention_fp8", "specdec_paged_attention_ex"):
+                return fn
+            return lambda *args: (flags.append(args[-2] & attention.EARLY_LAUNCH), fn(*args))[1]
+
+    s = case(F, [3, 3], [300, 40], seed=41)
+    k = torch.randn(s["c"].k_cache.shape[0], 256, 8, 128, device=DEV).bfloat16()
+
+    def go(tables, **where):
+        if cache == "e4m3":
+            c = s["c"]
+            return F.paged_attention_fp8(s["q"], c.k_cache, c.v_cache, c.k_scale, c.v_scale, tables, s["scale"],
+                                         early_launch=True, **where)
+        return attention.paged_attention(s["q"], k, k, tables, s["scale"], early_launch=True, **where)
+
+    varlen = dict(cu_seqlens_q=s["cu_q"], cu_seqlens_k=s["cu_k"], max_seqlen_q=3)
+    decode = dict(context_lens=s["ctx"], query_len_per_seq=3)
+    wide = torch.stack([s["ctx"], s["ctx"]], dim=1)[:, 0]
+    monkeypatch.setattr(_lib, "lib", lambda: Recorder())
+    want = go(s["tables"], **varlen)
+    outs = [go(s["tables"], **decode), go(s["tables"].long(), **varlen), go(s["tables"], **{**varlen, "cu_seqlens_q": s["cu_q"].long()}),
+            go(s["tables"], **{**varlen, "cu_seqlens_k": s["cu_k"].long()}), go(s["tables"], **{**decode, "context_lens": wide}),
+            go(s["tables"], **varlen, context_lens=wide)]
+    monkeypatch.undo()
+    assert flags == [1, 1, 0, 0, 0, 0, 1]
+    assert all(torch.equal(o, want) for o in outs) and device_error() == 0
+
+
 def test_attention_module_stores_then_attends(F):
     from nanovllm_b200.context import reset_context, set_context
     s = case(F, [8, 5], [600, 257], seed=34)

@@ -132,7 +132,9 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     if slot_mapping.numel() != N:
         raise ValueError(f"{slot_mapping.numel()} slots for {N} tokens")
     slots = _int32(slot_mapping)
-    call_on(index, _lib.lib().specdec_store_kvcache_fp8, key.data_ptr(), ks[0], value.data_ptr(), vs[0],
+    one_row = kv_heads * HEAD_DIM                           # a single row's stride says nothing
+    call_on(index, _lib.lib().specdec_store_kvcache_fp8, key.data_ptr(), ks[0] if N > 1 else one_row, value.data_ptr(),
+            vs[0] if N > 1 else one_row,
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), N, kv_heads,
             HEAD_DIM, blocks, block_size, group, Workspace.address(index, 256, "attention"), raw_stream(index))
 
@@ -174,17 +176,17 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError(f"max_ctas {max_ctas}: 0 (one CTA per SM) to 255")
     out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _output(out, shape, q.device)
     strides = q.stride()
-    if strides[2] != 1 or strides[1] != D or strides[0] % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-        strides = q.stride()
+    row_stride = strides[0] if T > 1 else H * D             # of one row it says nothing
+    if strides[2] != 1 or (H > 1 and strides[1] != D) or row_stride % 8 or q.data_ptr() % 16:
+        q, row_stride = q.clone(memory_format=torch.contiguous_format), H * D
     ws_bytes = _workspace_bytes(index, R, kv_heads)
     early_launch = early_launch and given_as_is((tables, block_tables), (cq, cu_seqlens_q), (ck, cu_seqlens_k),
                                                 (ctx, context_lens))
     flags = (EARLY_LAUNCH if early_launch else 0) | (max_ctas << CTAS_SHIFT)
-    call_on(index, _lib.lib().specdec_paged_attention_fp8, q.data_ptr(), T, strides[0], H, kv_heads, D,
+    call_on(index, _lib.lib().specdec_paged_attention_fp8, q.data_ptr(), T, row_stride, H, kv_heads, D,
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size, group,
             ptr(cq), ptr(ck), ptr(ctx), q_per_seq, R, tables.data_ptr(), tables.shape[1], max_q, scale, causal,
-            out.data_ptr(), out.stride(0), Workspace.address(index, ws_bytes, workspace), ws_bytes,
+            out.data_ptr(), out.stride(0) if T > 1 else H * D, Workspace.address(index, ws_bytes, workspace), ws_bytes,
             Workspace.address(index, 256, "attention"), flags, raw_stream(index))
     return out
 

@@ -328,6 +328,25 @@ def test_attention_strided_rows(F):
     assert torch.equal(out[:, 8:40], want) and (out[:, :8] == 3).all() and (out[:, 40:] == 3).all()
 
 
+def test_one_row_of_any_stride(F):
+    """The row stride of a single row (a slice of wider rows) says nothing: q, out, keys and values of an odd one; and a dense q
+    at an address that is no multiple of 16 bytes is copied."""
+    s = case(F, [1], [300], seed=40)
+    want = attend(F, s)
+    wide = torch.zeros(2, 32 * 128 + 4, dtype=torch.bfloat16, device=DEV)
+    wide[:1, :4096] = s["q"].view(1, -1)
+    q = wide.as_strided((1, 32, 128), (wide.stride(0), 128, 1))
+    out = torch.zeros(8200, dtype=torch.bfloat16, device=DEV).as_strided((1, 32, 128), (4100, 128, 1))
+    attend(F, dict(s, q=q), out=out)
+    assert torch.equal(out, want)
+    wide.view(-1)[4:4100] = s["q"].view(-1)
+    assert torch.equal(attend(F, dict(s, q=wide.view(-1)[4:4100].view(1, 32, 128))), want)
+    c = random_cache(F, 1, 128, 2, 16, 4)
+    key = torch.randn(1, 258, device=DEV).bfloat16().as_strided((1, 2, 128), (257, 128, 1))
+    check_store(F, c, key, key, torch.tensor([3], device=DEV, dtype=torch.int32), 16)
+    assert device_error() == 0
+
+
 def test_attention_is_the_same_every_time(F):
     lens = np.random.default_rng(5).integers(500, 3000, size=24).tolist()
     s = case(F, [8] * 24, lens, seed=31)

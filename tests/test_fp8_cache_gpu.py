@@ -130,6 +130,61 @@ def test_store_prompt_of_the_most_tokens(F):
                             torch.full((N + 1,), -1, device=DEV, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("N", [1184, 1185, 3333])
+@pytest.mark.parametrize("heads,group", [(1, 16), (8, 16), (9, 16), (2, 32), (9, 32)])
+def test_store_many_tokens_in_any_order(F, N, heads, group):
+    """Around and above the count where a CTA takes many tokens: slots shuffled over blocks, a fifth given twice, padding
+    between, slots past the cache, and a mapping that starts off a 16-byte boundary."""
+    from nanovllm_b200 import attention
+    block_size, blocks = 128, 40
+    c = random_cache(F, blocks, block_size, heads, group, N)
+    g = torch.Generator().manual_seed(N + heads)
+    first = N * 7 // 10
+    slots = torch.randperm(blocks * block_size, generator=g)[:first].to(torch.int32)
+    again = slots[torch.randperm(first, generator=g)[:N // 5]]
+    rest = torch.full((N - first - again.numel(),), -1, dtype=torch.int32)
+    rest[::9] = blocks * block_size + 5
+    slots = torch.cat([slots, again, rest])
+    slots = slots[torch.randperm(N, generator=g)]
+    mapping = torch.zeros(N + 1, dtype=torch.int32, device=DEV)
+    mapping[1:] = slots
+    key, value = rows(N, heads, N)
+    check_store(F, c, key, value, mapping[1:], group)
+    assert device_error() == 3
+    attention.reset_device_error(DEV)
+
+
+@pytest.mark.parametrize("group", [16, 32])
+@pytest.mark.parametrize("heads", [1, 8, 9])
+def test_store_runs_of_many_tokens(F, heads, group):
+    """Prompts one after another and verified rows of 8, each from the middle of a group, 2,500 tokens in a call."""
+    lens = [900, 1, 700, 17] + [8] * 110 + [2]
+    blocks = 64
+    c = random_cache(F, blocks, 128, heads, group, 19)
+    slots, at = [], 5
+    for n in lens:
+        slots += list(range(at, at + n))
+        at += n + 13
+    assert at <= blocks * 128
+    slots = torch.tensor(slots, dtype=torch.int32, device=DEV)
+    key, value = rows(slots.numel(), heads, 20)
+    check_store(F, c, key, value, slots, group)
+    assert device_error() == 0
+
+
+def test_store_rows_of_a_group_far_apart(F):
+    """Sixteen passes over 200 groups, each pass one slot of every group in another order: a group's tokens lie in many CTAs, and
+    group numbers 1024 apart (which the look over the slots does not tell apart at first) are all there."""
+    groups = [i + 1024 * (i % 3) for i in range(200)]
+    c = random_cache(F, 200, 256, 2, 16, 21)
+    g = torch.Generator().manual_seed(3)
+    slots = torch.cat([torch.tensor([16 * groups[j] + (o + j) % 16 for j in torch.randperm(200, generator=g).tolist()])
+                       for o in range(16)]).to(torch.int32).to(DEV)
+    key, value = rows(slots.numel(), 2, 22)
+    check_store(F, c, key, value, slots, 16)
+    assert device_error() == 0
+
+
 def test_store_nothing(F):
     c = random_cache(F, 1, 128, 2, 16, 13)
     before = [t.clone() for t in (c.k_cache.view(torch.uint8), c.v_cache.view(torch.uint8), c.k_scale, c.v_scale)]

@@ -17,10 +17,13 @@
 //   S^T[128 keys x 2*32] = K . [q1 | q2]^T   q = 2^e (q1 + q2 / 16), both e4m3: bf16's 8 bits are 4 + 4, so the split is
 //                                            exact down to 2^-14 of the item's largest query element (beyond: an absolute
 //                                            2^-22 of it), e from that element
-//   O^T[128 dims x 3*32] += V^T . [p1 | p2 | p3]^T   p = p1 + p2 + p3, all e5m2: 3 bits each, p to 2^-9 of itself (what
-//                                            bf16 gives) down to 2^-24 of the column's running maximum (e5m2's range)
+//   O^T[128 dims x 3*32] += V^T . [p1 | p2 | p3]^T   p = p1 + p2 / 8 + p3 / 64, all e5m2: 3 bits each, what is left over
+//                                            taken 8 times, so that each part has e5m2's whole range: off by 2^-9 of p (what
+//                                            bf16 gives) or, below 2^-21 of the column's running maximum, 2^-30 of that
 // N-wise parts read A once; stacked along K they would read it 2 and 3 times, and A's reads of shared memory are what an
-// MMA with so few columns costs.  The parts' sums are taken in fp32 after TMEM.
+// MMA with so few columns costs.  The parts' sums are taken in fp32 after TMEM.  (Parts on one scale cost 1 % less, 354 for
+// 357 us at 16k contexts, and lost what is below 2^-24 of the maximum: 1 % of a row of 262,144 keys, one of them e^17 times
+// as likely as each other, in one piece.  The denominator sums p itself.)
 // The scales never touch the codes: ks_j multiplies the score, and vs_j goes into the exponent: with t_j = s_j + log2 vs_j
 // the running maximum is over t, the tensor core gets p'_j = 2^(t_j - m) (so the largest contribution keeps every bit
 // whatever the scales' spread), and the denominator sums p'_j / vs_j.
@@ -587,8 +590,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           // ---- probabilities, column sums, and this group's 16 columns of row `row` of the parts (S(u) seen: PV(u-2) has
-          // released the buffer).  An fp16 pattern's high byte is its value cut to e5m2; what is left over is exact in
-          // fp16.  Two cuts, then the third part to nearest: fp16's 2^-12 and e5m2's last half step, 2^-9 of p', off it.
+          // released the buffer).  An fp16 pattern's high byte is its value cut to e5m2; what is left over, less than a
+          // quarter of it, is exact in fp16, and 8 times that stays below 2^15 as p' does.  Two cuts, then the third part to
+          // nearest: fp16's 2^-12 and e5m2's last half step off it, 2^-9 of p' or 2^-17 / 64.
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (i == 1 && !two) break;
@@ -602,6 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               l_part[j + 1] = l2.y;
               ph[j / 2] = __floats2half2_rn(p2.x, p2.y);
             }
+            const __half2 eight = bits_half2(0x48004800u);
             unsigned char* prow = sP + (buf * 2 + i) * kPBytes + row * kCols + (wg ^ ((row >> 2) & 1)) * 16;
 #pragma unroll
             for (int part = 0; part < kPParts; ++part) {
@@ -613,8 +618,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   lo += 0x00800080u;
                   hi += 0x00800080u;
                 } else {
-                  ph[2 * k] = __hsub2(ph[2 * k], bits_half2(lo & 0xff00ff00u));
-                  ph[2 * k + 1] = __hsub2(ph[2 * k + 1], bits_half2(hi & 0xff00ff00u));
+                  ph[2 * k] = __hmul2(__hsub2(ph[2 * k], bits_half2(lo & 0xff00ff00u)), eight);
+                  ph[2 * k + 1] = __hmul2(__hsub2(ph[2 * k + 1], bits_half2(hi & 0xff00ff00u)), eight);
                 }
                 wd[k] = __byte_perm(lo, hi, 0x7531);
               }
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_32x32b_2x16(tmem_o, tmem_o + kCols, o, o2);
         tmem_ld_32x32b_x16(tmem_o + 2 * kCols, o3);
 #pragma unroll
-        for (int j = 0; j < kGroupCols; ++j) o[j] += o2[j] + o3[j];
+        for (int j = 0; j < kGroupCols; ++j) o[j] = fmaf(o3[j], 1.0f / 64.0f, fmaf(o2[j], 0.125f, o[j]));
       }
       tc_fence_before();
       __syncwarp();

@@ -321,6 +321,37 @@ def test_attention_long_rows(F, k_lens):
     check(F, case(F, [8] * len(k_lens), k_lens, H=8, heads=2, seed=len(k_lens)))
 
 
+@pytest.fixture(scope="module")
+def long_row(F):
+    """262,144 zero keys but the first, which has a 1 in its first dim; values between 0.75 and 1.25."""
+    n = 1 << 18
+    c = F.FP8Cache.allocate(n // 256, 256, 1, DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    for at in range(0, n, 16384):
+        k = torch.zeros(16384, 1, 128, device=DEV)
+        k[0, 0, 0] = float(at == 0)
+        v = 0.75 + 0.5 * torch.rand(k.shape, device=DEV, generator=g)
+        F.store_kvcache_fp8(k.bfloat16(), v.bfloat16(), c.k_cache, c.v_cache, c.k_scale, c.v_scale,
+                            torch.arange(at, at + 16384, dtype=torch.int32, device=DEV))
+    return c, n
+
+
+@pytest.mark.parametrize("spike", [11.0, 12.5, 13.0, 13.5, 14.0, 14.5, 15.0, 15.5, 16.0, 16.5, 17.0, 17.5, 18.0, 19.0, 20.0])
+def test_attention_long_flat_tail_below_one_key(F, long_row, spike):
+    """One key e^spike times as likely as each of 262,143 others, which are 1 to 80 % of the row together, in one piece (a CTA for
+    the whole row keeps one running maximum): probabilities between 2^-16 and 2^-29 of the largest count as exactly as others."""
+    c, n = long_row
+    q = torch.zeros(1, 4, 128, device=DEV)
+    q[:, :, 0] = spike
+    s = dict(c=c, q=q.bfloat16(), tables=torch.arange(n // 256, dtype=torch.int32, device=DEV)[None], q_lens=[1], k_lens=[n],
+             cu_q=torch.tensor([0, 1], dtype=torch.int32, device=DEV), cu_k=torch.tensor([0, n], dtype=torch.int32, device=DEV),
+             scale=1.0)
+    out = attend(F, s, max_ctas=1)
+    want, spread = oracle(s)
+    assert device_error() == 0
+    agree(out, want, spread)
+
+
 @pytest.mark.parametrize("sharp,spread", [(0.001, 0.5), (20.0, 0.5), (300.0, 2.0), (1.0, 6.0)])
 def test_attention_flat_and_peaked(F, sharp, spread):
     """Scores from almost equal to far apart, groups of very different scales side by side."""

@@ -18,9 +18,11 @@
 // has a slot there; the leader's CTA looks over the call's slots (4 bytes a token, from L1 / L2) for the group's members and
 // does the whole group, so each group and its scales are written by one CTA.  A CTA takes some consecutive tokens, and one
 // of K and V (blockIdx.y); a warp takes a head's rows of a group into registers, 16 loads in flight.
-// Measured (8 KV heads, groups of 16): 16,000 tokens of four prompts 26 us, 98.5 MB at 3.8 TB/s: 6 us of it
-// the look over the slots, then bound by instructions fetched and issued for the rows (prefetching the rows into L2 during
-// the look 27.6 us).  512 verified tokens of 64 rows take 6.6 us and one token 3.4 us, bound by the launch and the dependent reads
+// Measured (8 KV heads, groups of 16): 16,000 tokens of four prompts 26 us, 98.5 MB at 3.8 TB/s (70 MB of them cross to DRAM
+// inside the launch: the codes stay in L2): 6 us of it the look over the slots, then bound by instructions fetched and issued
+// for the rows (prefetching the rows into L2 during the look 27.6 us).  Groups of 32 take 26 us too.  A warp keeps to one head
+// of eight, so fewer heads leave warps idle: 4, 2 and 1 heads 20, 19 and 17 us (groups of 32: 19, 16 and 14), where the bytes
+// are worth 7.6, 3.8 and 1.9.  512 verified tokens of 64 rows take 6.6 us and one token 3.4 us, bound by the launch and the dependent reads
 // (slot, members, rows, and the old codes where a scale rises).
 #include "common.cuh"
 #include "sm100.cuh"

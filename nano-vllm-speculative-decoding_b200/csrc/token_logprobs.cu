@@ -11,13 +11,18 @@
 // sum (x - m) e^(x - m) in fp32: nothing of the row is kept.  For the alternatives, the CTA's 64 groups of four threads
 // tell their maxima: those are 64 elements of its part, so their num_top-th largest is at most the part's, and only the
 // threads whose own maximum reaches it read their elements again (from L2): some 24 candidates for 20 alternatives
-// whatever the row.  Where ties bring more than the list holds, the part's alternatives are found one by one, a pass each.
+// where no value is shared by many.  Where ties bring more than the list holds, the part's alternatives are found one by one,
+// a pass each.  So does a row that a mask leaves fewer tokens than alternatives in some part, or has in fewer than num_top
+// groups: its bound is the mask's value.  With 5 tokens of 151,936 left and 20 alternatives, 8 rows take 59 us, 64 rows 370 and
+// 512 rows 2440 (unmasked 14, 18 and 46); with 1000 left 16, 28 and 92 behind -inf (the threads that saw nothing else look
+// again) and 14, 18 and 46 behind the type's lowest value.
 // The CTA that finishes a row last (a ticket that wraps itself; nobody waits) merges the parts in their order.  Clusters
 // with distributed shared memory in place of the tickets took 137 us where this takes 44.5 us (512 rows): their barriers
 // kept every CTA of a row until its slowest.
-// Measured at 151,936 tokens: 512 bf16 rows (480 of them asked for) with 20 alternatives 44.5 us (146 MB at 3.3 TB/s), 8
-// rows 10.4 us; 288 fp32 rows of 50,257 tokens without alternatives 14.2 us (3.8 TB/s).  Between the floor and these: a
-// row's chain of bound, second reads, ranking and merge, some 6 us, which only other CTAs' rows cover.
+// Measured at 151,936 tokens: 512 bf16 rows (480 of them asked for) with 20 alternatives 44.5 to 47 us (146 MB at 3.2 TB/s),
+// 8 rows with 5 10 to 11.5 us; 288 fp32 rows of 50,257 tokens without alternatives 14 to 15 us (3.7 TB/s).  Between the floor
+// and these: a row's chain of bound, second reads, ranking and merge, some 6 us, which only other CTAs' rows cover, and 480
+// live rows on 148 SMs being 3 or 4 each (1.23 times an equal share).
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -384,8 +389,9 @@ __global__ void __launch_bounds__(kThreads, 5)
 }
 
 // CTAs a row: enough for three an SM over the rows, each thread left at least four vectors; one where the rows do that alone.
-// (64 rows with 5 alternatives: 17.3, 16.3, 17.8, 18.1 and 23.3 us with 1, 2, 3, 4 and 6 an SM; 288 fp32 rows 35.8, 32.7,
-// 32.6, 40.8 and 37.0; 512 rows with 20 45.5 to three, then 56.)
+// (64 bf16 rows of 151,936 with 5 alternatives: 15.5, 15.2, 16.5, 16.9 and 20.8 us with 1, 2, 3, 4 and 6 an SM; 288 fp32 rows
+// of 151,936 without 36.0, 32.8, 32.8, 40.3 and 37.0, of 50,257 15.3, 14.8, 14.8, 18.9 and 18.3; 512 bf16 rows of 151,936 with
+// 20 45.8 to three, then 57.)
 static int parts_of(long long rows, long long V, int dtype, int sm_count) {
   const long long vectors = V / (16 / (long long)dtype_bytes(dtype));
   const long long wanted = (3LL * sm_count + rows - 1) / rows, most = vectors / (kThreads * 4);

@@ -22,11 +22,14 @@
 //                                            bf16 gives) or, below 2^-21 of the column's running maximum, 2^-30 of that
 // N-wise parts read A once; stacked along K they would read it 2 and 3 times, and A's reads of shared memory are what an
 // MMA with so few columns costs.  The parts' sums are taken in fp32 after TMEM.  (Parts on one scale cost 1 % less, 354 for
-// 357 us at 16k contexts, and lost what is below 2^-24 of the maximum: 1 % of a row of 262,144 keys, one of them e^17 times
-// as likely as each other, in one piece.  The denominator sums p itself.)
+// 357 us at 16k contexts, 424 for 430 sustained, and lost what is below 2^-24 of the maximum: 1 % of a row of 262,144 keys,
+// one of them e^17 times as likely as each other, in one piece.  The denominator sums p itself.  Taking the leftovers 8 times
+// only for long rows, behind a branch: 432 us.)
 // The scales never touch the codes: ks_j multiplies the score, and vs_j goes into the exponent: with t_j = s_j + log2 vs_j
 // the running maximum is over t, the tensor core gets p'_j = 2^(t_j - m) (so the largest contribution keeps every bit
-// whatever the scales' spread), and the denominator sums p'_j / vs_j.
+// whatever the scales' spread), and the denominator sums p'_j / vs_j.  (fp32's range bounds the spread: a key whose vs is
+// 2^-110 of another's can be missing from the denominator, where it counts 2^-23 of that other's weight or, only past 2^110,
+// more.)
 //   warp 0       TMA producer: K tiles and the scales  warps 4-11   softmax over keys (a TMEM lane is a key; two groups of
 //   warp 1       TMEM allocator, MMA issuer                          16 columns each), P parts, O rescale, epilogue
 //   warp 2       prologue                              warps 12-15  query parts of the next items; rows without keys
@@ -38,13 +41,14 @@
 // independent tiles' arithmetic to interleave (16k contexts: 379 -> 362 us; one tile ahead in software instead: 595 us).
 // The MMA warp runs converged with a predicated leader lane: issued from a divergent lane an MMA cost about 100 clocks,
 // more than its execution (429 -> 376 us).  Rings deeper than this lost time (5 stages of K and V: 15 % at 3k contexts).
-// Measured (32 query and 8 KV heads): 64 rows of 1 to 8 queries on 16k contexts 347 to 367 us (2144 MB, 0.90 to 0.95 of the
-// copy rate; the bf16 kernel on its cache 630 to 674 us) where the SMs hold 1.9 GHz; called for seconds on end the GPU
-// reaches its 1000 W and the clock falls to 1.5 to 1.7 GHz: 390 to 430 us, a pair's 2700 clocks being the softmax's chain
-// then.  64 draft blocks of 7 on 3k 88 us (97 sustained), 32 rows on 1k 30 us, one token on 1000 keys 12 us: what an item
-// costs beside its tiles (query parts, first wait, pieces and their merge).  At one clock and without gain: a warp each for
-// the score and the PV MMAs (the softmax then waits for P's buffer itself: 371 against 354 us), and 8 columns a
-// group for items of at most 16 (352 against 347 us: the chain is latency, not columns).
+// Measured (32 query and 8 KV heads, in a graph): 64 rows of 1 to 8 queries on 16k contexts 355 to 367 us (2144 MB, 0.90 to
+// 0.93 of the copy rate; the bf16 kernel on its cache 630 to 674 us) where the SMs hold 1.9 GHz; called for seconds on end
+// the GPU reaches its 1000 W and the clock falls to 1.5 to 1.7 GHz: 424 to 432 us (0.77), a pair's 2700 clocks being the
+// softmax's chain then.  64 draft blocks of 7 on 3k 88 to 92 us (95 sustained), 32 rows on 1k 30 us, one token on 1000 keys
+// 13 us: what an item costs beside its tiles (query parts, first wait, pieces and their merge).  Four of the softmax's
+// registers spill; their reloads are in its loop, some 6 a pair of tiles, 0.6 % of the instructions executed.  At one clock
+// and without gain: a warp each for the score and the PV MMAs (the softmax then waits for P's buffer itself: 371 against
+// 354 us), and 8 columns a group for items of at most 16 (352 against 347 us: the chain is latency, not columns).
 #include "paged_items.cuh"
 #include "specdec_b200.h"
 

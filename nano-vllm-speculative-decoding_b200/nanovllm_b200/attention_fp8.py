@@ -24,8 +24,16 @@ twice holds its last token.  The scales must be positive (FP8Cache starts them a
 
 Shapes and limits of the attention are those of nanovllm_b200.attention: head_dim 128, GQA groups of 1, 2, 4 or 8, rows of
 at most 32 / (H / Hkv) queries, block_size a multiple of 128.  A query that sees no key (a row with no context, or fewer
-keys than queries) gives zeros.  Errors found on the device are in attention.device_error: 2 row metadata, 3 a slot past
-the cache, 5 a block id outside the cache (read as block 0).
+keys than queries) gives zeros.  A NaN among a row's stored values reaches all of the row's queries, those whose mask
+leaves its key out too, as in the bf16 cache's attention (0 * NaN in the matrix product); a NaN key only those that see it.
+
+Accuracy: the queries of a row that share a KV head share an exponent, the largest element's, and are exact to 2^-22 of that
+element; probabilities are off by 2^-9 of themselves or 2^-30 of the largest one; sums are fp32.  The scales of a row's values
+may be up to 2^110 apart (a group of zeros has 2^-100): further apart, keys with the smaller ones can go missing from the
+softmax's sum.
+
+Errors found on the device are in attention.device_error: 2 row metadata, 3 a slot past the cache, 5 a block id outside the
+cache (read as block 0).
 """
 from __future__ import annotations
 
